@@ -456,3 +456,60 @@ def attention_quantize_int8(q8, q_sf, k8, k_sf, v8, v_sf, q, k, v, layout):
                                                x[0].data_ptr(), _I64x4(*x[0].stride()), x[1].data_ptr(), _I64x4(*x[1].stride()),
                                                x[2].data_ptr(), _I64x4(*x[2].stride()), None, None, B, H, Nq, Nkv, D, Dv, _stream(q)),
               "attention_quantize_int8")
+
+
+NORM_PRECISIONS = {None: 0, "fp8e4m3": 1, "nvfp4": 2}
+
+
+def rms_norm(out, sf, normed, residual_out, x, weight, residual, eps, precision=None, global_scale=None):
+    """Residual addition and RMS norm of the rows of x (no counterpart in the reference): out = (x + residual) / rms * weight, in bf16, in
+    e4m3 with the row scales `sf` (fp32 [align16(M)]), or in NVFP4 for `global_scale` with the block scales `sf` (either layout); normed:
+    None or the bf16 result beside a quantised one; residual_out: None or x + residual, in residual's type."""
+    _require(precision in NORM_PRECISIONS, f"Unsupported precision: {precision}")
+    _require(isinstance(x, torch.Tensor) and x.is_cuda and x.dtype == torch.bfloat16, "x must be a bfloat16 CUDA tensor")
+    _require(x.dim() == 2 and x.stride(1) == 1, "x must be a 2d matrix with contiguous rows")
+    M, K = x.shape
+    _require(K >= 1, "x must have at least one column")
+    _require(weight is None or isinstance(weight, torch.Tensor), "weight must be a tensor")
+    if weight is not None:
+        _require(weight.dtype in (torch.bfloat16, torch.float32), "weight must be bfloat16 or float")
+        _check_tensor(weight, weight.dtype, "weight")
+        _require(list(weight.shape) == [K], f"weight must have shape [{K}]")
+    if residual is not None:
+        _require(isinstance(residual, torch.Tensor) and residual.is_cuda and residual.dtype in (torch.bfloat16, torch.float32),
+                 "residual must be a bfloat16 or float CUDA tensor")
+        _require(list(residual.shape) == [M, K] and residual.stride(1) == 1, f"residual must be [{M}, {K}] with contiguous rows")
+    _require(residual_out is None or residual is not None, "residual_out needs a residual")
+    if residual_out is not None:
+        _check_tensor(residual_out, residual.dtype, "residual_out")
+        _require(list(residual_out.shape) == [M, K], "residual_out has an invalid shape")
+    layout = SF_AC4K
+    if precision is None:
+        _check_tensor(out, torch.bfloat16, "out")
+        _require(list(out.shape) == [M, K], "out has an invalid shape")
+        _require(normed is None and sf is None, "normed and sf stand beside a quantised output")
+    elif precision == "fp8e4m3":
+        _check_tensor(out, torch.float8_e4m3fn, "out")
+        _check_tensor(sf, torch.float32, "sf")
+        _require(list(out.shape) == [M, _align_up(K, 16)] and list(sf.shape) == [_align_up(M, 16)], "out or sf has an invalid shape")
+    else:
+        kt = _ceil_div(K, 64)
+        _check_tensor(out, torch.uint8, "out")
+        _check_tensor(sf, torch.float8_e4m3fn, "sf")
+        _check_tensor(global_scale, torch.float32, "global_scale")
+        _require(global_scale.dim() == 0, "global_scale must be a scalar")
+        layout = SF_AC4K if sf.dim() == 3 else SF_TILE128X4
+        want = [kt, _align_up(M, 16), 4] if layout == SF_AC4K else [_ceil_div(M, 128), kt, 32, 4, 4]
+        _require(list(out.shape) == [M, kt * 32] and list(sf.shape) == want, "out or sf has an invalid shape")
+    if normed is not None:
+        _check_tensor(normed, torch.bfloat16, "normed")
+        _require(list(normed.shape) == [M, K], "normed has an invalid shape")
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    for t in (out, sf, normed, residual_out, weight, residual, global_scale):
+        _require(t is None or t.device == x.device, "all tensors must be on one device")
+    with torch.cuda.device(x.device):
+        check(LIB.ac4k_rms_norm(out.data_ptr(), ptr(sf), ptr(global_scale), NORM_PRECISIONS[precision], layout, ptr(normed), ptr(residual_out),
+                                x.data_ptr(), ptr(residual), 0 if residual is None else _DT[residual.dtype], ptr(weight),
+                                0 if weight is None else _DT[weight.dtype], float(eps), M, K, x.stride(0),
+                                0 if residual is None else residual.stride(0), _stream(x)),
+              "rms_norm")

@@ -1,5 +1,5 @@
 // The operators' host side in one native call each: argument checks, output allocation and launches of `quantize`, `linear`,
-// `linear_requant`, `attention` and `rope3d`.  Built by ac4k_kernel_b200/build.py (build_pybind) with the host compiler.
+// `linear_requant`, `attention`, `rope3d` and `rms_norm`.  Built by ac4k_kernel_b200/build.py (build_pybind) with the host compiler.
 //
 // Why: the Python wrappers cost 20 - 25 us per launch (argument checks, ctypes marshalling, the device guard), several
 // times the kernels of a small call: a decode layer, quantisation and GEMM, took 78 us of which the GPU worked 12.
@@ -23,6 +23,7 @@
 #include <cmath>
 #include <optional>
 #include <string>
+#include <vector>
 
 #include "ac4k_b200.h"
 
@@ -284,6 +285,78 @@ py::object rope3d(py::handle hx, py::handle hgrid, py::handle hfreqs, py::handle
   return given ? py::reinterpret_borrow<py::object>(hout) : py::cast(out);
 }
 
+// A matrix with contiguous rows, of one of two types
+std::optional<at::Tensor> rows_of(py::handle h, at::ScalarType a, at::ScalarType b, int64_t M, int64_t K) {
+  if (!THPVariable_CheckExact(h.ptr())) return std::nullopt;
+  const at::Tensor &t = THPVariable_Unpack(h.ptr());
+  if (!plain(t) || (t.scalar_type() != a && t.scalar_type() != b) || !same_shape(t, {M, K}) || t.stride(1) != 1) return std::nullopt;
+  return t;
+}
+
+py::object rms_norm(py::handle hx, py::handle hweight, py::handle heps, py::handle hresidual, py::handle hprecision, py::handle hscale, py::handle hkeep,
+                    py::handle hlayout) {
+  const auto x = tensor_of(hx, at::kBFloat16, 2, false);
+  const auto layout = text_of(hlayout);
+  if (!x || x->stride(1) != 1 || x->size(1) < 1 || !layout || (*layout != "ac4k" && *layout != "128x4") || !PyBool_Check(hkeep.ptr()) ||
+      !PyFloat_CheckExact(heps.ptr()))
+    return py::none();
+  const int64_t M = x->size(0), K = x->size(1);
+  const float eps = (float)PyFloat_AS_DOUBLE(heps.ptr());
+  const bool keep = hkeep.ptr() == Py_True, tiled = *layout == "128x4";
+  int precision = AC4K_NORM_BF16;
+  if (!hprecision.is_none()) {
+    const auto name = text_of(hprecision);
+    if (!name || (*name != "fp8e4m3" && *name != "nvfp4")) return py::none();
+    precision = *name == "nvfp4" ? AC4K_NORM_NVFP4 : AC4K_NORM_E4M3;
+  }
+  at::Tensor weight, residual, scale;
+  if (!hweight.is_none()) {
+    if (!THPVariable_CheckExact(hweight.ptr())) return py::none();
+    weight = THPVariable_Unpack(hweight.ptr());
+    if (!plain(weight) || (weight.scalar_type() != at::kBFloat16 && weight.scalar_type() != at::kFloat) || !same_shape(weight, {K}) ||
+        !weight.is_contiguous() || weight.device() != x->device())
+      return py::none();
+  }
+  if (!hresidual.is_none()) {
+    const auto r = rows_of(hresidual, at::kBFloat16, at::kFloat, M, K);
+    if (!r || r->device() != x->device()) return py::none();
+    residual = *r;
+  }
+  if (hscale.is_none() != (precision != AC4K_NORM_NVFP4) || (keep && precision == AC4K_NORM_BF16)) return py::none();
+  if (precision == AC4K_NORM_NVFP4 && (!scalar_of(hscale, &scale) || scale.device() != x->device())) return py::none();
+  const c10::cuda::CUDAGuard guard(x->device());
+  at::Tensor out, sf, normed, residual_out;
+  unlocked([&] {
+    const int64_t kt = ceil_div(K, 64);
+    if (precision == AC4K_NORM_BF16) {
+      out = empty({M, K}, at::kBFloat16, *x);
+    } else if (precision == AC4K_NORM_E4M3) {
+      out = empty({M, align_up(K, 16)}, at::kFloat8_e4m3fn, *x);
+      sf = empty({align_up(M, 16)}, at::kFloat, *x);
+    } else {
+      out = empty({M, kt * 32}, at::kByte, *x);
+      sf = tiled ? empty({ceil_div(M, 128), kt, 32, 4, 4}, at::kFloat8_e4m3fn, *x) : empty({kt, align_up(M, 16), 4}, at::kFloat8_e4m3fn, *x);
+    }
+    if (keep) normed = empty({M, K}, at::kBFloat16, *x);
+    if (residual.defined()) residual_out = empty({M, K}, residual.scalar_type(), *x);
+    auto ptr = [](const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; };
+    check(ac4k_rms_norm(out.data_ptr(), ptr(sf), static_cast<const float *>(ptr(scale)), precision, tiled ? AC4K_SF_TILE128X4 : AC4K_SF_AC4K, ptr(normed),
+                        ptr(residual_out), x->data_ptr(), ptr(residual), residual.defined() ? dt_code(residual.scalar_type()) : 0, ptr(weight),
+                        weight.defined() ? dt_code(weight.scalar_type()) : 0, eps, M, K, x->stride(0), residual.defined() ? residual.stride(0) : 0,
+                        stream_of(*x)),
+          "rms_norm");
+  });
+  std::vector<py::object> made{py::cast(out)};
+  if (sf.defined()) made.push_back(py::cast(sf));
+  if (scale.defined()) made.push_back(py::reinterpret_borrow<py::object>(hscale));
+  if (normed.defined()) made.push_back(py::cast(normed));
+  if (residual_out.defined()) made.push_back(py::cast(residual_out));
+  if (made.size() == 1) return made[0];
+  py::tuple all(made.size());
+  for (size_t i = 0; i < made.size(); ++i) all[i] = made[i];
+  return std::move(all);
+}
+
 py::object attention(py::handle hq, py::handle hk, py::handle hv, py::handle hlayout, py::handle hprecision, py::handle hout) {
   const auto layout = text_of(hlayout), precision = text_of(hprecision);
   if (!layout || !precision) return py::none();
@@ -375,4 +448,5 @@ PYBIND11_MODULE(_host_calls, m) {
   m.def("linear_requant", &linear_requant);
   m.def("rope3d", &rope3d);
   m.def("attention", &attention);
+  m.def("rms_norm", &rms_norm);
 }

@@ -254,6 +254,22 @@ int ac4k_mha_int8_x_fp8_fwd(void *O, const int64_t o_stride[4], const void *Q, c
 int ac4k_rope3d(void *out, const void *x, const int32_t *grid_sizes, const void *freqs, int64_t B, int64_t S,
                 int64_t N, int64_t D, int64_t max_pos, ac4k_stream_t stream);
 
+/* The residual's addition and the RMS norm of M rows of K elements, in front of a linear layer (no counterpart in the reference):
+ *   s = x + residual,  v = s / sqrt(mean(s^2) + eps) * weight,  residual_out = s,  out = v
+ * in fp32, each output rounded once from it (the norm takes s as it was added up, not as residual_out holds it; a quantised out takes v).
+ *   x: bf16, rows x_stride elements apart; residual: NULL, or bf16 / fp32 (residual_dtype), rows residual_stride elements apart;
+ *   weight: NULL (ones) or K values of bf16 / fp32 (weight_dtype).
+ *   out: AC4K_NORM_BF16 bf16 [M, K]; AC4K_NORM_E4M3 e4m3 [M, align16(K)] with sf fp32 [align16(M)], the row's largest |v| / 448 (what
+ *   ac4k_quantize_fp8 emits; a row whose largest |v| is below 2^-117 has scale and codes 0); AC4K_NORM_NVFP4 packed [M, align64(K) / 2]
+ *   with block scales sf in `sf_layout` for the given global scale (what ac4k_linear_nvfp4 takes).  Padding is written as zeros.
+ *   normed: NULL, or v in bf16 [M, K] beside a quantised out.  residual_out: NULL or [M, K] of residual_dtype; it may be the residual
+ *   itself (residual_stride = K) or x (x_stride = K, bf16), and overlaps no tensor of the call otherwise.
+ * K <= 32768.  Sums of squares past fp32's range (elements of 1e17 and more) give zeros, as infinity under the root does. */
+enum { AC4K_NORM_BF16 = 0, AC4K_NORM_E4M3 = 1, AC4K_NORM_NVFP4 = 2 };
+int ac4k_rms_norm(void *out, void *sf, const float *global_scale, int precision, int sf_layout, void *normed, void *residual_out,
+                  const void *x, const void *residual, int residual_dtype, const void *weight, int weight_dtype, float eps,
+                  int64_t M, int64_t K, int64_t x_stride, int64_t residual_stride, ac4k_stream_t stream);
+
 /* Device buffers that the other processes of the node can map (CUDA IPC), for the destinations of
  * ac4k_linear_nvfp4_gather.  No counterpart in the reference.
  *   ac4k_peer_alloc: cudaMalloc on the current device + its 64-byte IPC handle.
