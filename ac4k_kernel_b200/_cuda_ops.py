@@ -513,3 +513,45 @@ def rms_norm(out, sf, normed, residual_out, x, weight, residual, eps, precision=
                                 0 if weight is None else _DT[weight.dtype], float(eps), M, K, x.stride(0),
                                 0 if residual is None else residual.stride(0), _stream(x)),
               "rms_norm")
+
+
+def _check_rows(x, dtypes, name):
+    _require(isinstance(x, torch.Tensor) and x.is_cuda, f"{name} must be a CUDA tensor")
+    _require(x.dtype in dtypes, f"Inconsistency of Tensor type: {name} is {x.dtype}")
+    _require(x.dim() == 2 and (x.size(1) <= 1 or x.stride(1) == 1), f"{name} must be a 2d matrix with contiguous rows")
+
+
+def lora(out, y, x, a, b, offsets, adapters, scaling=None):
+    """out = y + scaling[j] * (x A_j^T) B_j^T for the rows of each request and its adapter j (no counterpart in the reference).  y, out:
+    [T, N] bf16, fp16 or fp32; x: bf16 [T, K]; a: bf16 [adapters, R, K]; b: bf16 [adapters, N, R]; offsets: int32 [requests + 1];
+    adapters: int32 [requests], negative for none; scaling: None or fp32 [adapters].  out may be y."""
+    _check_rows(y, tuple(_DT), "y")
+    _check_rows(out, (y.dtype,), "out")
+    _check_rows(x, (torch.bfloat16,), "x")
+    T, N = y.shape
+    _require(list(out.shape) == [T, N], "out must have the shape of y")
+    _require(x.size(0) == T, f"x size(0) must be {T} but see {x.size(0)}")
+    K = x.size(1)
+    _check_tensor(a, torch.bfloat16, "a")
+    _check_tensor(b, torch.bfloat16, "b")
+    _require(a.dim() == 3 and a.size(2) == K, f"a must be [adapters, rank, {K}]")
+    L, R = a.size(0), a.size(1)
+    _require(list(b.shape) == [L, N, R], f"b must be [{L}, {N}, {R}]")
+    _check_tensor(adapters, torch.int32, "adapters")
+    _require(adapters.dim() == 1, "adapters must be a vector")
+    S = adapters.size(0)
+    _check_tensor(offsets, torch.int32, "offsets")
+    _require(list(offsets.shape) == [S + 1], f"offsets must have shape [{S + 1}]")
+    if scaling is not None:
+        _check_tensor(scaling, torch.float32, "scaling")
+        _require(list(scaling.shape) == [L], f"scaling must have shape [{L}]")
+    for t in (out, x, a, b, offsets, adapters, scaling):
+        _require(t is None or t.device == y.device, "all tensors must be on one device")
+    with torch.cuda.device(y.device):
+        need = ctypes.c_int64(0)
+        check(LIB.ac4k_lora_workspace(T, S, K, N, R, ctypes.byref(need)), "lora")
+        ws = torch.empty((need.value // 4,), dtype=torch.float32, device=y.device)
+        check(LIB.ac4k_lora(out.data_ptr(), y.data_ptr(), _DT[y.dtype], x.data_ptr(), a.data_ptr(), b.data_ptr(), offsets.data_ptr(),
+                            adapters.data_ptr(), None if scaling is None else scaling.data_ptr(), ws.data_ptr(), need.value, T, S, L, K, N, R,
+                            x.stride(0), y.stride(0), out.stride(0), _stream(y)),
+              "lora")

@@ -1,5 +1,5 @@
 // The operators' host side in one native call each: argument checks, output allocation and launches of `quantize`, `linear`,
-// `linear_requant`, `attention`, `rope3d` and `rms_norm`.  Built by ac4k_kernel_b200/build.py (build_pybind) with the host compiler.
+// `linear_requant`, `attention`, `rope3d`, `rms_norm` and `lora`.  Built by ac4k_kernel_b200/build.py (build_pybind) with the host compiler.
 //
 // Why: the Python wrappers cost 20 - 25 us per launch (argument checks, ctypes marshalling, the device guard), several
 // times the kernels of a small call: a decode layer, quantisation and GEMM, took 78 us of which the GPU worked 12.
@@ -285,6 +285,44 @@ py::object rope3d(py::handle hx, py::handle hgrid, py::handle hfreqs, py::handle
   return given ? py::reinterpret_borrow<py::object>(hout) : py::cast(out);
 }
 
+// out = y + the requests' adapters
+py::object lora(py::handle hy, py::handle hx, py::handle ha, py::handle hb, py::handle hoffsets, py::handle hadapters, py::handle hscaling, py::handle hout) {
+  if (!THPVariable_CheckExact(hy.ptr())) return py::none();
+  const at::Tensor &y = THPVariable_Unpack(hy.ptr());
+  const auto x = tensor_of(hx, at::kBFloat16, 2, false), a = tensor_of(ha, at::kBFloat16, 3), b = tensor_of(hb, at::kBFloat16, 3);
+  const auto offsets = tensor_of(hoffsets, at::kInt, 1), adapters = tensor_of(hadapters, at::kInt, 1);
+  if (!plain(y) || dt_code(y.scalar_type()) < 0 || y.dim() != 2 || !x || !a || !b || !offsets || !adapters) return py::none();
+  const int64_t T = y.size(0), N = y.size(1), K = x->size(1), L = a->size(0), R = a->size(1), S = adapters->size(0);
+  if (y.stride(1) != 1 || x->stride(1) != 1 || x->size(0) != T || a->size(2) != K || !same_shape(*b, {L, N, R}) || offsets->size(0) != S + 1) return py::none();
+  at::Tensor scaling, out;
+  if (!hscaling.is_none()) {
+    const auto t = tensor_of(hscaling, at::kFloat, 1);
+    if (!t || t->size(0) != L) return py::none();
+    scaling = *t;
+  }
+  if (!hout.is_none()) {
+    if (!THPVariable_CheckExact(hout.ptr())) return py::none();
+    out = THPVariable_Unpack(hout.ptr());
+    if (!plain(out) || out.scalar_type() != y.scalar_type() || !same_shape(out, {T, N}) || out.stride(1) != 1 || out.device() != y.device()) return py::none();
+  }
+  for (const at::Tensor *t : {&*x, &*a, &*b, &*offsets, &*adapters})
+    if (t->device() != y.device()) return py::none();
+  if (scaling.defined() && scaling.device() != y.device()) return py::none();
+  const c10::cuda::CUDAGuard guard(y.device());
+  unlocked([&] {
+    if (!out.defined()) out = empty({T, N}, y.scalar_type(), y);
+    int64_t bytes = 0;
+    check(ac4k_lora_workspace(T, S, K, N, R, &bytes), "lora");
+    const at::Tensor ws = empty({bytes / 4}, at::kFloat, y);
+    check(ac4k_lora(out.data_ptr(), y.data_ptr(), dt_code(y.scalar_type()), x->data_ptr(), a->data_ptr(), b->data_ptr(),
+                    static_cast<const int32_t *>(offsets->data_ptr()), static_cast<const int32_t *>(adapters->data_ptr()),
+                    scaling.defined() ? static_cast<const float *>(scaling.data_ptr()) : nullptr, ws.data_ptr(), bytes, T, S, L, K, N, R, x->stride(0),
+                    y.stride(0), out.stride(0), stream_of(y)),
+          "lora");
+  });
+  return hout.is_none() ? py::cast(out) : py::reinterpret_borrow<py::object>(hout);
+}
+
 // A matrix with contiguous rows, of one of two types
 std::optional<at::Tensor> rows_of(py::handle h, at::ScalarType a, at::ScalarType b, int64_t M, int64_t K) {
   if (!THPVariable_CheckExact(h.ptr())) return std::nullopt;
@@ -449,4 +487,5 @@ PYBIND11_MODULE(_host_calls, m) {
   m.def("rope3d", &rope3d);
   m.def("attention", &attention);
   m.def("rms_norm", &rms_norm);
+  m.def("lora", &lora);
 }

@@ -270,6 +270,22 @@ int ac4k_rms_norm(void *out, void *sf, const float *global_scale, int precision,
                   const void *x, const void *residual, int residual_dtype, const void *weight, int weight_dtype, float eps,
                   int64_t M, int64_t K, int64_t x_stride, int64_t residual_stride, ac4k_stream_t stream);
 
+/* Low-rank adapters of a batch of requests, added to the output of a projection that all of them share (no counterpart in the
+ * reference).  The rows [offsets[i], offsets[i + 1]) are those of request i:
+ *   out[t] = y[t] + scaling[j] * B_j (A_j x[t])  with j = adapters[i];  out[t] = y[t] where j is negative or no adapter (j >= n_adapters) and
+ *   for rows in front of offsets[0] and behind offsets[requests].
+ *   x: bf16 [rows, K], y and out: y_dtype [rows, N], all with contiguous rows that are *_stride elements apart; out is y itself (with its
+ *   stride) or overlaps it nowhere.  a: bf16 [n_adapters, R, K], b: bf16 [n_adapters, N, R], dense; an adapter of a lower rank has zeros
+ *   behind it.  offsets: int32 [requests + 1], ascending within [0, rows]; adapters: int32 [requests]; scaling: fp32 [n_adapters] or NULL
+ *   (ones); all on the device.  R <= 128.
+ * A x is held in fp32 and its product with B in fp32 with 16 bits of each value of A x; one rounding to out.
+ * workspace: as many bytes as ac4k_lora_workspace says for the current device, 16-byte aligned, for this call alone (contents undefined). */
+int ac4k_lora_workspace(int64_t rows, int64_t requests, int64_t K, int64_t N, int64_t R, int64_t *bytes);
+int ac4k_lora(void *out, const void *y, int y_dtype, const void *x, const void *a, const void *b, const int32_t *offsets,
+              const int32_t *adapters, const float *scaling, void *workspace, int64_t workspace_bytes, int64_t rows, int64_t requests,
+              int64_t n_adapters, int64_t K, int64_t N, int64_t R, int64_t x_stride, int64_t y_stride, int64_t out_stride,
+              ac4k_stream_t stream);
+
 /* Device buffers that the other processes of the node can map (CUDA IPC), for the destinations of
  * ac4k_linear_nvfp4_gather.  No counterpart in the reference.
  *   ac4k_peer_alloc: cudaMalloc on the current device + its 64-byte IPC handle.
