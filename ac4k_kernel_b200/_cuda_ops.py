@@ -555,3 +555,40 @@ def lora(out, y, x, a, b, offsets, adapters, scaling=None):
                             adapters.data_ptr(), None if scaling is None else scaling.data_ptr(), ws.data_ptr(), need.value, T, S, L, K, N, R,
                             x.stride(0), y.stride(0), out.stride(0), _stream(y)),
               "lora")
+
+
+def linear_nvfp4_grouped(D, A, A_sf, A_global_scale, B, B_sf, B_global_scale, offsets, bias=None, fill=False):
+    """D = (A_gs * B_gs[e]) * A @ B[e]^T + bias[e] for the rows [offsets[e], offsets[e + 1]) of each group e (no counterpart in the
+    reference).  A: packed [M, K/2], A_sf [K/64, align16(M), 4]; B: packed [E, N, K/2], B_sf [E, K/64, align16(N), 4]; B_global_scale: a
+    scalar or [E]; offsets: int32 [E + 1]; bias: None or [E, N]; fill: write zeros to the rows of no group."""
+    _require(isinstance(D, torch.Tensor) and D.is_cuda and D.dim() == 2 and D.is_contiguous(), "d must be a contiguous 2d CUDA matrix")
+    _require(D.dtype in _DT, "d must be bfloat16, half or float")
+    M, N = D.shape
+    _check_tensor(A, torch.uint8, "a")
+    _check_tensor(B, torch.uint8, "b")
+    _require(A.dim() == 2 and A.size(0) == M, f"a must be a 2d matrix of {M} rows")
+    _require(B.dim() == 3 and B.size(1) == N and B.size(2) == A.size(1), f"b must be [groups, {N}, {A.size(1)}]")
+    E, K = B.size(0), A.size(1) * 2
+    kt = _ceil_div(K, 64)
+    _check_tensor(A_sf, torch.float8_e4m3fn, "scale_a")
+    _check_tensor(B_sf, torch.float8_e4m3fn, "scale_b")
+    _require(list(A_sf.shape) == [kt, _align_up(M, 16), 4], "scale_a has an invalid shape")
+    _require(list(B_sf.shape) == [E, kt, _align_up(N, 16), 4], "scale_b has an invalid shape")
+    _check_tensor(A_global_scale, torch.float32, "global_scale_a")
+    _require(A_global_scale.dim() == 0, "A_global_scale must be a scalar")
+    _check_tensor(B_global_scale, torch.float32, "global_scale_b")
+    _require(B_global_scale.dim() == 0 or list(B_global_scale.shape) == [E], "B_global_scale must be a scalar or one value per group")
+    _check_tensor(offsets, torch.int32, "offsets")
+    _require(list(offsets.shape) == [E + 1], f"offsets must have shape [{E + 1}]")
+    if bias is not None:
+        _require(isinstance(bias, torch.Tensor) and bias.dtype in _DT, "bias must be bfloat16, half or float")
+        _check_tensor(bias, bias.dtype, "bias")
+        _require(list(bias.shape) == [E, N], f"bias must have shape [{E}, {N}]")
+    for t in (A, A_sf, A_global_scale, B, B_sf, B_global_scale, offsets, bias):
+        _require(t is None or t.device == D.device, "all tensors must be on one device")
+    with torch.cuda.device(D.device):
+        check(LIB.ac4k_linear_nvfp4_grouped(D.data_ptr(), _DT[D.dtype], A.data_ptr(), A_sf.data_ptr(), A_global_scale.data_ptr(), B.data_ptr(),
+                                            B_sf.data_ptr(), B_global_scale.data_ptr(), int(B_global_scale.dim()),
+                                            None if bias is None else bias.data_ptr(), 0 if bias is None else _DT[bias.dtype], offsets.data_ptr(),
+                                            int(bool(fill)), M, E, N, K, _stream(D)),
+              "linear_nvfp4_grouped")

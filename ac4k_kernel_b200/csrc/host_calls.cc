@@ -1,5 +1,5 @@
 // The operators' host side in one native call each: argument checks, output allocation and launches of `quantize`, `linear`,
-// `linear_requant`, `attention`, `rope3d`, `rms_norm` and `lora`.  Built by ac4k_kernel_b200/build.py (build_pybind) with the host compiler.
+// `linear_grouped`, `linear_requant`, `attention`, `rope3d`, `rms_norm` and `lora`.  Built by ac4k_kernel_b200/build.py (build_pybind) with the host compiler.
 //
 // Why: the Python wrappers cost 20 - 25 us per launch (argument checks, ctypes marshalling, the device guard), several
 // times the kernels of a small call: a decode layer, quantisation and GEMM, took 78 us of which the GPU worked 12.
@@ -241,6 +241,41 @@ py::object linear(py::handle a, py::handle a_sf, py::handle a_gs, py::handle b, 
           "linear_nvfp4");
   });
   return out.is_none() ? py::cast(d) : py::reinterpret_borrow<py::object>(out);
+}
+
+py::object linear_grouped(py::handle ha, py::handle hasf, py::handle hags, py::handle hb, py::handle hbsf, py::handle hbgs, py::handle hoffsets,
+                          py::handle hbias, py::handle hout) {
+  const auto a = tensor_of(ha, at::kByte, 2), b = tensor_of(hb, at::kByte, 3), offsets = tensor_of(hoffsets, at::kInt, 1);
+  const auto a_sf = tensor_of(hasf, at::kFloat8_e4m3fn, 3), b_sf = tensor_of(hbsf, at::kFloat8_e4m3fn, 4), b_gs = tensor_of(hbgs, at::kFloat);
+  at::Tensor a_gs, bias, d;
+  if (!a || !b || !a_sf || !b_sf || !offsets || !b_gs || !scalar_of(hags, &a_gs)) return py::none();
+  const int64_t M = a->size(0), E = b->size(0), N = b->size(1), K = a->size(1) * 2, kt = ceil_div(K, 64);
+  if (b->size(2) != a->size(1) || !same_shape(*a_sf, {kt, align_up(M, 16), 4}) || !same_shape(*b_sf, {E, kt, align_up(N, 16), 4}) ||
+      !same_shape(*offsets, {E + 1}) || !(b_gs->dim() == 0 || same_shape(*b_gs, {E})))
+    return py::none();
+  if (!hbias.is_none()) {
+    if (!THPVariable_CheckExact(hbias.ptr())) return py::none();
+    bias = THPVariable_Unpack(hbias.ptr());
+    if (!plain(bias) || dt_code(bias.scalar_type()) < 0 || !bias.is_contiguous() || !same_shape(bias, {E, N}) || bias.device() != a->device()) return py::none();
+  }
+  if (!hout.is_none()) {
+    if (!THPVariable_CheckExact(hout.ptr())) return py::none();
+    d = THPVariable_Unpack(hout.ptr());
+    if (!plain(d) || !d.is_contiguous() || dt_code(d.scalar_type()) < 0 || !same_shape(d, {M, N}) || d.device() != a->device()) return py::none();
+  }
+  for (const at::Tensor *t : std::initializer_list<const at::Tensor *>{&*a_sf, &a_gs, &*b, &*b_sf, &*b_gs, &*offsets})
+    if (t->device() != a->device()) return py::none();
+  const c10::cuda::CUDAGuard guard(a->device());
+  unlocked([&] {
+    const bool fill = !d.defined();
+    if (fill) d = empty({M, N}, at::kBFloat16, *a);
+    check(ac4k_linear_nvfp4_grouped(d.data_ptr(), dt_code(d.scalar_type()), a->data_ptr(), a_sf->data_ptr(), static_cast<const float *>(a_gs.data_ptr()),
+                                    b->data_ptr(), b_sf->data_ptr(), static_cast<const float *>(b_gs->data_ptr()), (int)b_gs->dim(),
+                                    bias.defined() ? bias.data_ptr() : nullptr, bias.defined() ? dt_code(bias.scalar_type()) : 0,
+                                    static_cast<const int32_t *>(offsets->data_ptr()), fill ? 1 : 0, M, E, N, K, stream_of(*a)),
+          "linear_nvfp4_grouped");
+  });
+  return hout.is_none() ? py::cast(d) : py::reinterpret_borrow<py::object>(hout);
 }
 
 py::object linear_requant(py::handle a, py::handle a_sf, py::handle a_gs, py::handle b, py::handle b_sf, py::handle b_gs, py::handle out_gs,
@@ -486,6 +521,7 @@ PYBIND11_MODULE(_host_calls, m) {
   m.def("linear_requant", &linear_requant);
   m.def("rope3d", &rope3d);
   m.def("attention", &attention);
+  m.def("linear_grouped", &linear_grouped);
   m.def("rms_norm", &rms_norm);
   m.def("lora", &lora);
 }

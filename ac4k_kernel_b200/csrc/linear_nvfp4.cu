@@ -432,18 +432,7 @@ enum { kTmapOperand = 0, kTmapWords = 1, kTmapOut16 = 2, kTmapOperand64 = 3 };
 // kTmapOut16: 16-bit elements, 128-byte swizzle.
 // classes > 0: a rank-3 map {d0, ceil(d1 / 4), classes} with strides {4 * pitch, pitch}: coordinate (x, i, q) is row 4 i + q, and a
 // box {box0, box1, box2} lands in shared memory with q outermost.
-static int encode_cached(int kind, const void *ptr, int64_t d0, int64_t d1, int64_t pitch, int box0, int box1,
-                         CUtensorMap *out, int classes = 0, int box2 = 1) {
-  static std::mutex mu;
-  static std::vector<TmapEntry> cache;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  TmapKey key{ptr, d0, d1, pitch, box0, box1, kind, dev, classes, box2};
-  {
-    std::lock_guard<std::mutex> lk(mu);
-    for (auto &e : cache)
-      if (e.key == key) { *out = e.map; return 0; }
-  }
+static int encode(int kind, const void *ptr, int64_t d0, int64_t d1, int64_t pitch, int box0, int box1, int classes, int box2, CUtensorMap *out) {
   EncodeTiledFn enc = get_encode_fn();
   if (!enc) return fail(AC4K_ERR_DEVICE, "cuTensorMapEncodeTiled is not available from this driver");
   const bool bytes = kind == kTmapOperand || kind == kTmapOperand64;
@@ -462,12 +451,28 @@ static int encode_cached(int kind, const void *ptr, int64_t d0, int64_t d1, int6
     gstride[0] = (cuuint64_t)pitch * esize * 4;
     gstride[1] = (cuuint64_t)pitch * esize;
   }
-  CUtensorMap m;
-  CUresult r = enc(&m, dt, classes > 0 ? 3 : 2,
+  CUresult r = enc(out, dt, classes > 0 ? 3 : 2,
                    const_cast<void *>(ptr), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                    swz,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail((int)r > 0 ? (int)r : 999, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+  return 0;
+}
+
+static int encode_cached(int kind, const void *ptr, int64_t d0, int64_t d1, int64_t pitch, int box0, int box1,
+                         CUtensorMap *out, int classes = 0, int box2 = 1) {
+  static std::mutex mu;
+  static std::vector<TmapEntry> cache;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  TmapKey key{ptr, d0, d1, pitch, box0, box1, kind, dev, classes, box2};
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    for (auto &e : cache)
+      if (e.key == key) { *out = e.map; return 0; }
+  }
+  CUtensorMap m;
+  if (int e = encode(kind, ptr, d0, d1, pitch, box0, box1, classes, box2, &m)) return e;
   {
     std::lock_guard<std::mutex> lk(mu);
     if (cache.size() >= 64) cache.erase(cache.begin());
@@ -480,6 +485,10 @@ static int encode_cached(int kind, const void *ptr, int64_t d0, int64_t d1, int6
 // packed operand [rows, row_bytes]: boxes of 128 bytes x box_rows rows, 128-byte swizzle
 int get_tmap(const void *ptr, int64_t rows, int64_t row_bytes, int box_rows, CUtensorMap *out) {
   return encode_cached(kTmapOperand, ptr, row_bytes, rows, row_bytes, BKB, box_rows, out);
+}
+
+int make_tmap(const void *ptr, int64_t rows, int64_t row_bytes, int box_rows, CUtensorMap *out) {
+  return encode(kTmapOperand, ptr, row_bytes, rows, row_bytes, BKB, box_rows, 0, 1, out);
 }
 
 // Tiled scale factors [row blocks of 128][K/64][512 bytes] seen as a matrix of 512-byte rows: a box of

@@ -50,37 +50,6 @@ struct Cfg {
 };
 }  // namespace skinny
 
-__device__ __forceinline__ void st_shared_f32(uint32_t addr, float v) {
-  asm volatile("st.shared::cta.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
-}
-// bulk copy from this CTA's shared memory into the shared memory of a CTA of the cluster, completing (bytes) on an
-// mbarrier of that CTA; 16-byte aligned addresses and size
-__device__ __forceinline__ void bulk_copy_to_cluster(uint32_t dst_cluster_addr, uint32_t src, uint32_t bytes, uint32_t bar_cluster_addr) {
-  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(dst_cluster_addr), "r"(src), "r"(bytes), "r"(bar_cluster_addr) : "memory");
-}
-__device__ __forceinline__ float ld_shared_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cta.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
-
-template <int NT>
-__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[NT]) {
-  if constexpr (NT == 16) tmem_ld_32x32b_x16(taddr, r);
-  else if constexpr (NT == 32) tmem_ld_32x32b_x32(taddr, r);
-  else tmem_ld_32x32b_x64(taddr, r);
-  tmem_ld_wait();
-  tmem_pin(r);
-}
-
-template <int OUT_DT>
-__device__ __forceinline__ void store_out(typename OutT<OUT_DT>::type *dst, float v) {
-  if (OUT_DT == AC4K_DT_BF16) *dst = (typename OutT<OUT_DT>::type)__float2bfloat16_rn(v);
-  else if (OUT_DT == AC4K_DT_FP16) *dst = (typename OutT<OUT_DT>::type)__float2half_rn(v);
-  else *dst = (typename OutT<OUT_DT>::type)v;
-}
-
 // One K slice: the accumulator is the sum.  alpha, bias, round, store row by row, in groups of eight rows
 // (one row at a time with its own bound cost 10 ns a row: 4.25 against 3.46 us at 64 x 512 x 512, 5.56 against 4.78 at 64 x 20000 x 1024).
 template <int NT, int OUT_DT>

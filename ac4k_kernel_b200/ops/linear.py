@@ -10,6 +10,7 @@ from .. import _cuda_ops
 from ..native import host_calls
 
 linear_nvfp4 = _cuda_ops.linear_nvfp4
+linear_nvfp4_grouped = _cuda_ops.linear_nvfp4_grouped
 
 
 class Ac4kLinearOp(torch.nn.Module):
@@ -68,3 +69,23 @@ def linear_requant(x, x_scale, x_global_scale, weight, weight_scale, weight_glob
     _cuda_ops.linear_nvfp4_requant(out, out_sf, out_global_scale, x, x_scale, x_global_scale, weight,
                                    weight_scale, weight_global_scale, bias)
     return out, out_sf, out_global_scale
+
+
+def linear_grouped(x, x_scale, x_global_scale, weight, weight_scale, weight_global_scale, offsets, bias=None, out=None):
+    """`linear()` with a weight per group of rows, e.g. the experts of a layer on rows that are sorted by expert (the reference has no
+    counterpart): out[t] = x[t] @ weight[e].T + bias[e] for the rows offsets[e] to offsets[e + 1].
+
+    x, x_scale, x_global_scale: what `quantize(rows, 0, 1)` returns for all rows together, packed [M, K/2] u8, [K/64, align_up(M, 16), 4] e4m3,
+    0-dim; weight, weight_scale: `quantize(weights, 1, 2)` of the [E, N, K] weights, [E, N, K/2] u8, [E, K/64, align_up(N, 16), 4] e4m3;
+    weight_global_scale: 0-dim, or [E] where each weight was quantised by itself; offsets: int32 [E + 1], ascending; bias: [E, N]
+    bf16/fp16/fp32; out: optional [M, N] bf16/fp16/fp32.  A group may be empty.  Rows of no group (in front of offsets[0] or behind
+    offsets[E]) are zeros in an output that is allocated here and left as they are in one that is given.  Returns out."""
+    if host_calls is not None:
+        made = host_calls.linear_grouped(x, x_scale, x_global_scale, weight, weight_scale, weight_global_scale, offsets, bias, out)
+        if made is not None:
+            return made
+    fill = out is None
+    if out is None:
+        out = torch.empty((x.shape[0], weight.shape[1]), dtype=torch.bfloat16, device=x.device)
+    linear_nvfp4_grouped(out, x, x_scale, x_global_scale, weight, weight_scale, weight_global_scale, offsets, bias, fill)
+    return out

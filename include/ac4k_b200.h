@@ -286,6 +286,18 @@ int ac4k_lora(void *out, const void *y, int y_dtype, const void *x, const void *
               int64_t n_adapters, int64_t K, int64_t N, int64_t R, int64_t x_stride, int64_t y_stride, int64_t out_stride,
               ac4k_stream_t stream);
 
+/* ac4k_linear_nvfp4 with a weight per group of rows, e.g. the experts of a layer on rows that are sorted by expert (no counterpart in the
+ * reference): for the rows t of group e, [offsets[e], offsets[e + 1]),
+ *   D[t, n] = cast(A_gs * B_gs[e] * sum_k A[t, k] B[e, n, k] + bias[e, n])
+ *   A: [M, K/2] with A_sf [K/64, align16(M), 4] and one A_gs, as ac4k_quantize_nvfp4 emits them for the M rows together;
+ *   B: [groups, N, K/2] with B_sf [groups, K/64, align16(N), 4]; B_gs: one scalar, or [groups] where b_gs_per_group is not 0;
+ *   bias: NULL or [groups, N] of `bias_dtype`; offsets: int32 [groups + 1] on the device, ascending within [0, M]; D: [M, N] of `d_dtype`.
+ * A group may be empty and may begin at any row.  Rows of no group (in front of offsets[0], behind offsets[groups]) are written as zeros where
+ * `fill` is not 0 and left as they are otherwise.  K a multiple of 64; groups * N <= 2^30. */
+int ac4k_linear_nvfp4_grouped(void *D, int d_dtype, const void *A, const void *A_sf, const float *A_gs, const void *B, const void *B_sf,
+                              const float *B_gs, int b_gs_per_group, const void *bias, int bias_dtype, const int32_t *offsets, int fill,
+                              int64_t M, int64_t groups, int64_t N, int64_t K, ac4k_stream_t stream);
+
 /* Device buffers that the other processes of the node can map (CUDA IPC), for the destinations of
  * ac4k_linear_nvfp4_gather.  No counterpart in the reference.
  *   ac4k_peer_alloc: cudaMalloc on the current device + its 64-byte IPC handle.
