@@ -3,16 +3,19 @@
 //   out[t] = y[t] + scaling[a] * B_a (A_a x[t]),   a = adapters[request of row t], or none: out[t] = y[t]
 //
 // A rank of 8 to 128 makes 2 R operations per byte of x and of y, below what the memory allows for up to R = 64: the work is to read x, y and the
-// adapters once and to write out once.  Two launches: `shrink` leaves A x in fp32 (R values a row), `expand` adds B of it to y.  Both take a
+// adapters once and to write out once.  Two launches: `shrink` leaves A x (R values a row), `expand` adds B of it to y.  Both take a
 // tile of rows of one request against its adapter with mma.sync (16 x 8 x 16, bf16, fp32 accumulators): the tiles are small and ragged, no operand
-// is read twice from global memory by a warp, and what tcgen05 would add, rate, is not what bounds them.  Operands go from global memory
-// straight to registers in 16-byte vectors: a product's sum may run over k in any order, so a thread takes 8 neighbouring k of a row and
-// deals them to the two MMAs of a step of 32 k, the same for both operands; and the columns of `expand` are dealt so that the 8 results
+// is read twice from global memory by a warp, and what tcgen05 would add, rate, is not what bounds them.  Operands come through
+// rings in shared memory (cp.async), x and y each thread's own 16-byte vectors, the adapter's shared by the block: a product's sum may run
+// over k in any order, so a thread takes 8 neighbouring k of a row and deals them to the two MMAs of a step of 32 k, the same for both
+// operands, and needs no ldmatrix; the columns of `expand` are dealt so that the 8 results
 // of a thread over four MMAs are neighbours, which it loads from y and stores in vectors.
 //
-// A x is rounded to nothing less than fp32: `expand` splits it into two bf16 values (16 bits of mantissa together) and takes two MMAs.
-// With a few rows a request the K dimension of `shrink` is cut into slices, whose sums `expand` adds in order: no atomics, the same result each time.
+// A x is summed in fp32 and handed over as two bf16 values (16 bits of mantissa together), for which `expand` takes two MMAs.
+// K is cut into slices where there are few tiles; the slices of a tile are a cluster, which adds their sums in order: no atomics, the same result
+// each time, and `expand` reads 4 bytes a value (it read every slice's sums at first: 137 MB through L2 for 4099 rows of rank 64 in 7 slices).
 #include "ragged.cuh"
+#include "sm100_ptx.cuh"
 
 namespace ac4k {
 
@@ -26,7 +29,7 @@ struct Args {
   void *out;
   const int32_t *offsets, *adapters;
   const float *scaling;        // or NULL: ones
-  float *ws;                   // [slices][rows][RP]
+  uint32_t *ws;                // [rows][RP]: scaling * A x, a bf16 value (low half) and what it leaves of the fp32 one
   int64_t x_stride, y_stride, out_stride;
   int rows, requests, count;   // count: adapters
   int K, N, R;
@@ -35,21 +38,37 @@ struct Args {
   bool x_vec, a_vec, b_vec, y_vec;
 };
 
-// 8 elements of a row from `k` on; zeros at and behind `end`
-template <bool CS>
-__device__ __forceinline__ uint4 load8(const uint16_t *row, int k, int end, bool vec) {
-  uint4 v = make_uint4(0, 0, 0, 0);
+// 16 bytes of shared memory from 8 elements of a row, beginning at element k; zeros at and behind `end`.  Vectors (k and end multiples of 8,
+// 16-byte aligned) arrive asynchronously, single elements at once.
+__device__ __forceinline__ void stage8(uint32_t dst, const uint16_t *row, int k, int end, bool vec) {
   if (vec) {
-    if (k < end) v = CS ? __ldcs(reinterpret_cast<const uint4 *>(row + k)) : __ldg(reinterpret_cast<const uint4 *>(row + k));
+    const uint32_t bytes = k < end ? 16u : 0u;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(bytes ? row + k : row), "r"(bytes) : "memory");
   } else {
     uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (k + i < end) w[i >> 1] |= (uint32_t)__ldg(row + k + i) << (16 * (i & 1));
-    v = make_uint4(w[0], w[1], w[2], w[3]);
+    asm volatile("st.shared::cta.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
   }
+}
+__device__ __forceinline__ void stage16(uint32_t dst, const void *src, uint32_t bytes) {      // 16 bytes, those behind the first `bytes` zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void stage_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void stage_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared::cta.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ uint2 lds8(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared::cta.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t shared_addr(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -70,79 +89,165 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 }
 }  // namespace lora
 
+namespace lora {
+// `shrink`: what a stage of the ring holds.  KW: k of a warp in a stage; TM 64: all warps the same k, TM 16: in turn.
+template <int TM, int RP>
+struct Shrink {
+  static constexpr int KW = TM == 64 || RP <= 32 ? 64 : 32;
+  static constexpr int KB = TM == 64 ? KW : 4 * KW;             // k of the block
+  static constexpr int PARTS = KB / KW;
+  static constexpr int CH = KW / 8;                             // 16-byte chunks of a row
+  static constexpr int X_BYTES = kThreads * (KW / 32) * 2 * 16; // each thread its own two rows' chunks
+  static constexpr int A_PART = RP * KW * 2;
+  static constexpr int STAGE = X_BYTES + PARTS * A_PART;
+  static constexpr int D = TM == 64 ? 4 : (RP == 128 || RP == 32 ? 3 : 4);
+  static constexpr int SMEM = D * STAGE;
+  // chunk c of adapter row r: rows of 8 chunks lie with their halves exchanged in every other row, so that the eight threads of a phase
+  // (two rows, four chunks) meet all banks; two rows of 4 chunks do by themselves
+  static __device__ __forceinline__ uint32_t a_at(int r, int c) { return (uint32_t)(r * CH + (CH == 8 ? c ^ ((r & 1) << 2) : c)) * 16u; }
+};
+}  // namespace lora
+
 // A x: a block takes one tile of rows and one slice of K.  TM 64: a warp per 16 rows, all of the slice; TM 16 (a few rows a request): the
-// warps divide the slice's K steps, and the block adds their sums.
+// warps divide each stage's k, and the block adds their sums.  The adapter's rows are shared by the block, x by nobody: a
+// thread loads just what it feeds to its MMAs.
 template <int TM, int RP>
 __global__ void __launch_bounds__(lora::kThreads)
 lora_shrink_kernel(const lora::Args p) {
   using namespace lora;
+  using C = Shrink<TM, RP>;
   constexpr int NT = RP / 8;
+  extern __shared__ __align__(128) uint8_t smem[];
   __shared__ RaggedScratch scratch;
   grid_dependency_wait();
   grid_launch_dependents();
-  const RaggedTile tile = ragged_tile<kThreads>(p.offsets, p.requests, p.rows, TM, blockIdx.x, &scratch);
-  if (tile.group < 0) return;
+  const int slice = p.slices > 1 ? (int)ptx::cluster_ctarank() : 0;
+  const RaggedTile tile = ragged_tile<kThreads>(p.offsets, p.requests, p.rows, TM, blockIdx.x / p.slices, &scratch);
+  if (tile.group < 0) return;               // (the blocks of a cluster have the same tile)
   const int adapter = adapter_of(p, tile);
   if (adapter < 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int m0 = tile.row0 + (TM == 64 ? warp * 16 : 0);
-  const int k0 = blockIdx.y * p.k_slice, k1 = min(p.K, k0 + p.k_slice);
+  const int m0 = tile.row0 + (TM == 64 ? warp * 16 : 0), r0 = m0 + g, r1 = m0 + g + 8;
+  const int k0 = min(p.K, slice * p.k_slice), k1 = min(p.K, k0 + p.k_slice);
+  const bool live0 = r0 < tile.row1, live1 = r1 < tile.row1;
+  const uint16_t *x0 = p.x + (int64_t)(live0 ? r0 : tile.row0) * p.x_stride, *x1 = p.x + (int64_t)(live1 ? r1 : tile.row0) * p.x_stride;
+  const uint16_t *a = p.a + (int64_t)adapter * p.R * p.K;
+  const uint32_t base = shared_addr(smem);
+  const int part = TM == 64 ? 0 : warp;
   float acc[NT][4];
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
-  if (m0 < tile.row1) {
-    const int r0 = m0 + g, r1 = m0 + g + 8;
-    const uint16_t *x0 = p.x + (int64_t)r0 * p.x_stride, *x1 = p.x + (int64_t)r1 * p.x_stride;
-    const int end0 = r0 < tile.row1 ? k1 : 0, end1 = r1 < tile.row1 ? k1 : 0;
-    const uint16_t *a = p.a + (int64_t)adapter * p.R * p.K;
-    constexpr int U = RP <= 32 ? 4 : 2;          // steps of 32 k whose loads are in flight together
-    constexpr int STEP = TM == 64 ? 32 : 32 * 4;
-#pragma unroll 1
-    for (int k = k0 + (TM == 64 ? 0 : warp * 32); k < k1; k += STEP * U) {
-      uint4 xa[U], xb[U], w[U][NT];
+  // A stage, from k on.  In whole vectors a thread has its places worked out once: its two rows of x, and of the adapter one row in every ROWS, which
+  // move on by a stage's k each time (worked out anew for each load, a stage of rank 32 took 294 instructions a warp, 16 of them MMAs: 50 us
+  // for 8192 x 8192, and the memory idle two thirds of the time).
+  constexpr int LOADS = RP * C::CH * C::PARTS / kThreads, ROWS = kThreads / C::CH;
+  static_assert(RP % ROWS == 0, "a thread's loads lie in one column of chunks");
+  const int a_c = threadIdx.x % C::CH, a_r = threadIdx.x / C::CH;
+  const uint16_t *xp0 = x0 + k0 + part * C::KW + 8 * t, *xp1 = x1 + k0 + part * C::KW + 8 * t;
+  const uint16_t *ap = a + (int64_t)a_r * p.K + k0 + a_c * 8;
+  const int64_t a_rows = (int64_t)ROWS * p.K;
+  const uint32_t x_to = base + threadIdx.x * 16, a_to = base + C::X_BYTES + C::a_at(a_r, a_c);
+  const uint32_t bytes0 = live0 ? 16 : 0, bytes1 = live1 ? 16 : 0;
+  auto fill = [&](uint32_t off, int k) {
+    if (p.x_vec && p.a_vec && k + C::KB <= k1) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int kk = k + u * STEP + 8 * t;
-        xa[u] = load8<true>(x0, kk, end0, p.x_vec);
-        xb[u] = load8<true>(x1, kk, end1, p.x_vec);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const int r = 8 * j + g;
-          w[u][j] = load8<false>(a + (int64_t)r * p.K, kk, r < p.R ? k1 : 0, p.a_vec);
-        }
+      for (int u = 0; u < C::KW / 32; ++u) {
+        stage16(x_to + off + (2 * u) * kThreads * 16, xp0 + u * 32, bytes0);
+        stage16(x_to + off + (2 * u + 1) * kThreads * 16, xp1 + u * 32, bytes1);
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          mma_bf16(acc[j], xa[u].x, xb[u].x, xa[u].y, xb[u].y, w[u][j].x, w[u][j].y);
-          mma_bf16(acc[j], xa[u].z, xb[u].z, xa[u].w, xb[u].w, w[u][j].z, w[u][j].w);
-        }
+      for (int i = 0; i < LOADS; ++i) {
+        const int r = i * ROWS % RP, q = i * ROWS / RP;
+        stage16(a_to + off + q * C::A_PART + r * C::CH * 16, ap + (r / ROWS) * a_rows + q * C::KW, a_r + r < p.R ? 16 : 0);
+      }
+      xp0 += C::KB;
+      xp1 += C::KB;
+      ap += C::KB;
+      return;
     }
+#pragma unroll
+    for (int u = 0; u < C::KW / 32; ++u) {
+      const int kk = k + part * C::KW + u * 32 + 8 * t;
+      stage8(x_to + off + (2 * u) * kThreads * 16, x0, kk, live0 ? k1 : 0, p.x_vec);
+      stage8(x_to + off + (2 * u + 1) * kThreads * 16, x1, kk, live1 ? k1 : 0, p.x_vec);
+    }
+#pragma unroll 1
+    for (int i = threadIdx.x; i < RP * C::CH * C::PARTS; i += kThreads) {
+      const int q = i / (RP * C::CH), r = i / C::CH % RP, c = i % C::CH;
+      stage8(base + off + C::X_BYTES + q * C::A_PART + C::a_at(r, c), a + (int64_t)(r < p.R ? r : 0) * p.K, k + q * C::KW + c * 8, r < p.R ? k1 : 0, p.a_vec);
+    }
+  };
+  const int steps = (k1 - k0 + C::KB - 1) / C::KB;
+#pragma unroll
+  for (int i = 0; i < C::D - 1; ++i) {
+    if (i < steps) fill(i * C::STAGE, k0 + i * C::KB);
+    stage_commit();
   }
-  float *ws = p.ws + (int64_t)blockIdx.y * p.rows * RP;
-  if (TM == 64) {
+  uint32_t now = 0, next = (C::D - 1) * C::STAGE;         // stages that are read and filled
+  const uint32_t x_at = base + threadIdx.x * 16, a_at0 = base + C::X_BYTES + part * C::A_PART + C::a_at(g, t);
+  const uint32_t a_at1 = base + C::X_BYTES + part * C::A_PART + C::a_at(g, C::CH == 8 ? 4 + t : t);
+#pragma unroll 1
+  for (int i = 0; i < steps; ++i) {
+    stage_wait<C::D - 2>();
+    __syncthreads();              // stage i is there for all, and all are done with the one that is filled next
+    if (i + C::D - 1 < steps) fill(next, k0 + (i + C::D - 1) * C::KB);
+    stage_commit();
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      if (m0 + g < tile.row1) *reinterpret_cast<float2 *>(ws + (int64_t)(m0 + g) * RP + 8 * j + 2 * t) = make_float2(acc[j][0], acc[j][1]);
-      if (m0 + g + 8 < tile.row1) *reinterpret_cast<float2 *>(ws + (int64_t)(m0 + g + 8) * RP + 8 * j + 2 * t) = make_float2(acc[j][2], acc[j][3]);
-    }
-  } else {
-    __shared__ __align__(16) float sums[4][16][RP];
+    for (int u = 0; u < C::KW / 32; ++u) {
+      const uint4 xa = lds16(x_at + now + (2 * u) * kThreads * 16), xb = lds16(x_at + now + (2 * u + 1) * kThreads * 16);
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      *reinterpret_cast<float2 *>(&sums[warp][g][8 * j + 2 * t]) = make_float2(acc[j][0], acc[j][1]);
-      *reinterpret_cast<float2 *>(&sums[warp][g + 8][8 * j + 2 * t]) = make_float2(acc[j][2], acc[j][3]);
+      for (int j = 0; j < NT; ++j) {
+        const uint4 w = lds16((u ? a_at1 : a_at0) + now + j * 8 * C::CH * 16);
+        mma_bf16(acc[j], xa.x, xb.x, xa.y, xb.y, w.x, w.y);
+        mma_bf16(acc[j], xa.z, xb.z, xa.w, xb.w, w.z, w.w);
+      }
     }
-    __syncthreads();
-    const int n = (tile.row1 - tile.row0) * RP;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const int m = i / RP, r = i % RP;
-      ws[(int64_t)(tile.row0 + m) * RP + r] = (sums[0][m][r] + sums[1][m][r]) + (sums[2][m][r] + sums[3][m][r]);
-    }
+    now = now + C::STAGE == C::D * C::STAGE ? 0 : now + C::STAGE;
+    next = next + C::STAGE == C::D * C::STAGE ? 0 : next + C::STAGE;
   }
+  // The sums of this block's slice, [row of the tile][RP], then those of all slices: the blocks of the cluster take a share of the values each, add
+  // them in the order of the slices, scale and round them to two bf16 parts.
+  float *sums = reinterpret_cast<float *>(smem);
+  constexpr int WARPS = TM == 64 ? 1 : 4;               // sums of a row
+  static_assert(WARPS * TM * RP * 4 <= C::SMEM, "the sums reuse the ring");
+  stage_wait<0>();
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    float *d = sums + (warp * 16 + g) * RP + 8 * j + 2 * t;
+    *reinterpret_cast<float2 *>(d) = make_float2(acc[j][0], acc[j][1]);
+    *reinterpret_cast<float2 *>(d + 8 * RP) = make_float2(acc[j][2], acc[j][3]);
+  }
+  if (p.slices > 1) ptx::cluster_sync();
+  else __syncthreads();
+  const float scale = p.scaling != nullptr ? __ldg(p.scaling + adapter) : 1.0f;
+  const int n = (tile.row1 - tile.row0) * RP;
+  uint32_t *ws = p.ws + (int64_t)tile.row0 * RP;
+  for (int i = (slice * kThreads + threadIdx.x) * 4; i < n; i += p.slices * kThreads * 4) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int q = 0; q < p.slices; ++q) {
+      const uint32_t at = p.slices > 1 ? ptx::map_to_cta(base + i * 4, q) : base + i * 4;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        float4 d;
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(d.x), "=f"(d.y), "=f"(d.z), "=f"(d.w) : "r"(at + w * 16 * RP * 4) : "memory");
+        v.x += d.x; v.y += d.y; v.z += d.z; v.w += d.w;
+      }
+    }
+    const float f[4] = {v.x, v.y, v.z, v.w};
+    uint32_t u[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      // (behind the rank: not 0 * infinity, which is what an infinity in x has left there)
+      const float a = i % RP + e < p.R ? __fmul_rn(f[e], scale) : 0.0f;
+      const float h = __bfloat162float(__float2bfloat16_rn(a));
+      u[e] = pack_bf16(h, isfinite(h) ? __fsub_rn(a, h) : 0.0f);        // (the difference is exact)
+    }
+    *reinterpret_cast<uint4 *>(ws + i) = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+  if (p.slices > 1) ptx::cluster_sync();                // no block leaves while another still reads its sums
 }
 
 namespace lora {
@@ -157,7 +262,6 @@ template <> struct Row8<__nv_bfloat16> {
   static __device__ __forceinline__ void store(void *p, const float (&f)[8]) {
     *reinterpret_cast<uint4 *>(p) = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
   }
-  static __device__ __forceinline__ float get(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
   static __device__ __forceinline__ __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
 };
 template <> struct Row8<__half> {
@@ -176,7 +280,6 @@ template <> struct Row8<__half> {
     for (int i = 0; i < 4; ++i) { const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]); u[i] = *reinterpret_cast<const uint32_t *>(&h); }
     *reinterpret_cast<uint4 *>(p) = make_uint4(u[0], u[1], u[2], u[3]);
   }
-  static __device__ __forceinline__ float get(const __half *p) { return __half2float(*p); }
   static __device__ __forceinline__ __half put(float v) { return __float2half_rn(v); }
 };
 template <> struct Row8<float> {
@@ -188,19 +291,37 @@ template <> struct Row8<float> {
     reinterpret_cast<float4 *>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
     reinterpret_cast<float4 *>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
   }
-  static __device__ __forceinline__ float get(const float *p) { return *p; }
   static __device__ __forceinline__ float put(float v) { return v; }
 };
 
-// 8 neighbouring values of a row, the first at column n: from memory, or as far as they lie in front of N
+// 8 neighbouring values of a row, the first at column n, into this thread's places of the ring (16 bytes each, kThreads apart); those at and
+// behind N: zeros or nothing
 template <typename T>
-__device__ __forceinline__ void load_y(const T *row, int n, int N, bool vec, float (&f)[8]) {
+__device__ __forceinline__ void stage_y(uint32_t dst, const T *row, int n, int N, bool live, bool vec) {
+  constexpr int PARTS = sizeof(T) / 2;
+  if (!live) return;
   if (vec) {
-    if (n < N) Row8<T>::load(row + n, f);
-  } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) if (n + i < N) f[i] = Row8<T>::get(row + n + i);
+    for (int i = 0; i < PARTS; ++i)
+      if (n < N) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + i * kThreads * 16), "l"(row + n + 8 / PARTS * i) : "memory");
+  } else {
+    T v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = n + i < N ? row[n + i] : T(0.0f);
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(v);
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i)
+      asm volatile("st.shared::cta.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + i * kThreads * 16), "r"(w[4 * i]), "r"(w[4 * i + 1]), "r"(w[4 * i + 2]),
+                   "r"(w[4 * i + 3]) : "memory");
   }
+}
+template <typename T>
+__device__ __forceinline__ void staged_y(uint32_t src, float (&f)[8]) {
+  constexpr int PARTS = sizeof(T) / 2;
+  uint4 v[PARTS];
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) v[i] = lds16(src + i * kThreads * 16);
+  Row8<T>::load(v, f);
 }
 // the same values bit for bit
 template <typename T>
@@ -225,119 +346,179 @@ __device__ __forceinline__ void store_y(T *row, int n, int N, bool vec, const fl
 }
 }  // namespace lora
 
+namespace lora {
+// `expand`: what a stage of the ring holds: the rows of B of NC columns, and y's values for each thread's results
+template <int TM, int RP, typename T>
+struct Expand {
+  static constexpr int UNITS = TM == 64 ? 2 : 1;                // of 32 columns, for each warp
+  static constexpr int NC = TM == 64 ? 64 : 128;
+  static constexpr int CH = RP / 8;
+  static constexpr int B_BYTES = NC * RP * 2;
+  static constexpr int Y_UNIT = kThreads * (int)sizeof(T) * 8;  // one row's values of a unit
+  static constexpr int STAGE = B_BYTES + UNITS * 2 * Y_UNIT;
+  static constexpr int D = RP == 128 ? 3 : 4;
+  static constexpr int SMEM = D * STAGE;
+  // chunk c of B's row n.  The eight threads of a phase read four chunks of rows n, n + 1: as in Shrink.  Rank 16: sixteen threads read halves
+  // of chunks of rows n, n + 1, n + 8, n + 9; pairs of rows change places in every other eight.
+  static __device__ __forceinline__ uint32_t b_at(int n, int c) {
+    if (RP == 16) return (uint32_t)((n ^ (((n >> 3) & 1) << 1)) * 2 + c) * 16u;
+    return (uint32_t)(n * CH + (CH >= 8 ? c ^ ((n & 1) << 2) : c)) * 16u;
+  }
+};
+}  // namespace lora
+
 // y + B (A x): a block takes one tile of rows and n_block columns, a warp 16 rows and 32 columns at a time.  TM 64: the warps have 16 rows each,
 // the same columns; TM 16: the same rows, columns in turn.
 template <int TM, int RP, typename T>
 __global__ void __launch_bounds__(lora::kThreads)
 lora_expand_kernel(const lora::Args p) {
   using namespace lora;
+  using C = Expand<TM, RP, T>;
   constexpr int KC = RP / 32 > 0 ? RP / 32 : 1;      // steps of 32 k (one of 16 for rank 16)
+  extern __shared__ __align__(128) uint8_t smem[];
   __shared__ RaggedScratch scratch;
   // The offsets, y and the adapters may be read in front of the wait: the shrink kernel's blocks let this one in behind their own wait, so
   // all that was enqueued before them is complete.
   const RaggedTile tile = ragged_tile<kThreads>(p.offsets, p.requests, p.rows, TM, blockIdx.x, &scratch);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int adapter = tile.group == -2 ? -1 : adapter_of(p, tile);
-  const int m0 = tile.row0 + (TM == 64 ? warp * 16 : 0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int n_first = blockIdx.y * p.n_block, n_end = min(p.N, n_first + p.n_block);
+  const int m0 = tile.row0 + (TM == 64 ? warp * 16 : 0), column = TM == 64 ? 0 : warp * 32;
   const bool live0 = tile.group != -2 && m0 + g < tile.row1, live1 = tile.group != -2 && m0 + g + 8 < tile.row1;
   const T *y0 = static_cast<const T *>(p.y) + (int64_t)(m0 + g) * p.y_stride, *y1 = y0 + 8 * p.y_stride;
   T *o0 = static_cast<T *>(p.out) + (int64_t)(m0 + g) * p.out_stride, *o1 = o0 + 8 * p.out_stride;
-  const int n_first = blockIdx.y * p.n_block + (TM == 64 ? 0 : warp * 32), n_end = min(p.N, (int)(blockIdx.y + 1) * p.n_block);
-  constexpr int NSTEP = TM == 64 ? 32 : 128;
   if (tile.group == -2 || adapter < 0) {
     grid_dependency_wait();
     grid_launch_dependents();
     if (tile.group == -2 || p.out == p.y) return;
-    for (int n = n_first; n < n_end; n += NSTEP) {     // rows without an adapter
+    for (int n = n_first + column; n < n_end; n += TM == 64 ? 32 : 128) {     // rows without an adapter
       if (live0) copy8<T>(o0, y0, n + 8 * t, p.N, p.y_vec);
       if (live1) copy8<T>(o1, y1, n + 8 * t, p.N, p.y_vec);
     }
     return;
   }
+  const uint16_t *b = p.b + (int64_t)adapter * p.N * p.R;
+  const uint32_t base = shared_addr(smem);
+  // A stage, from column n on; whole vectors of whole columns as in `shrink`
+  constexpr int LOADS = C::NC * C::CH / kThreads, COLS = kThreads / C::CH;
+  const int b_c = threadIdx.x % C::CH, b_n = threadIdx.x / C::CH;
+  const uint16_t *bp = b + (int64_t)(n_first + b_n) * p.R + b_c * 8;
+  const int64_t b_cols = (int64_t)COLS * p.R, b_step = (int64_t)C::NC * p.R;
+  const T *yp0 = y0 + n_first + column + 8 * t, *yp1 = y1 + n_first + column + 8 * t;
+  const uint32_t b_to = base + C::b_at(b_n, b_c), y_to = base + C::B_BYTES + threadIdx.x * 16, b_bytes = b_c * 8 < p.R ? 16 : 0;
+  auto fill = [&](uint32_t off, int n) {
+    if (p.b_vec && p.y_vec && n + C::NC <= p.N) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) stage16(b_to + off + i * COLS * C::CH * 16, bp + i * b_cols, b_bytes);
+#pragma unroll
+      for (int u = 0; u < C::UNITS; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (h ? live1 : live0) {
+#pragma unroll
+            for (int q = 0; q < (int)sizeof(T) / 2; ++q)
+              stage16(y_to + off + (2 * u + h) * C::Y_UNIT + q * kThreads * 16, (h ? yp1 : yp0) + 32 * u + q * (16 / (int)sizeof(T)), 16);
+          }
+      bp += b_step;
+      yp0 += C::NC;
+      yp1 += C::NC;
+      return;
+    }
+#pragma unroll 1
+    for (int i = threadIdx.x; i < C::NC * C::CH; i += kThreads) {
+      const int col = i / C::CH, c = i % C::CH;
+      const bool in = n + col < p.N;
+      stage8(base + off + C::b_at(col, c), b + (int64_t)(in ? n + col : 0) * p.R, c * 8, in ? p.R : 0, p.b_vec);
+    }
+#pragma unroll
+    for (int u = 0; u < C::UNITS; ++u) {
+      const int col = n + column + 32 * u + 8 * t;
+      stage_y<T>(y_to + off + 2 * u * C::Y_UNIT, y0, col, p.N, live0, p.y_vec);
+      stage_y<T>(y_to + off + (2 * u + 1) * C::Y_UNIT, y1, col, p.N, live1, p.y_vec);
+    }
+  };
+  const int steps = (n_end - n_first + C::NC - 1) / C::NC;
+#pragma unroll
+  for (int i = 0; i < C::D - 1; ++i) {
+    if (i < steps) fill(i * C::STAGE, n_first + i * C::NC);
+    stage_commit();
+  }
   grid_dependency_wait();
   grid_launch_dependents();
-  if (m0 >= tile.row1) return;
-  // A x of this warp's rows, the slices added in order, scaled and split into two bf16 parts: the fragments of a step of 32 k hold
-  // k = 8 t + {0, 1}, {2, 3} (first MMA) and {4, 5}, {6, 7} (second); rank 16: k = 4 t + {0, 1}, {2, 3}
+  // Both parts of A x for this warp's rows: the fragments of a step of 32 k hold k = 8 t + {0, 1}, {2, 3} (first MMA) and {4, 5}, {6, 7} (second);
+  // rank 16: k = 4 t + {0, 1}, {2, 3}.  Pair i -> MMA i / 2, k half i % 2; registers {row g, row g + 8} x {k half}
   uint32_t hi[KC][2][4], lo[KC][2][4];
-  const float scale = p.scaling != nullptr ? __ldg(p.scaling + adapter) : 1.0f;
   constexpr int PER = RP == 16 ? 4 : 8;
 #pragma unroll
   for (int c = 0; c < KC; ++c)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float v[PER];
+      uint4 v[PER / 4];
 #pragma unroll
-      for (int i = 0; i < PER; ++i) v[i] = 0.0f;
-      if (h ? live1 : live0) {
-        const float *w = p.ws + (int64_t)(m0 + g + 8 * h) * RP + c * 32 + PER * t;
-        for (int s = 0; s < p.slices; ++s, w += (int64_t)p.rows * RP) {
+      for (int q = 0; q < PER / 4; ++q) {
+        v[q] = make_uint4(0, 0, 0, 0);
+        if (h ? live1 : live0) v[q] = *reinterpret_cast<const uint4 *>(p.ws + (int64_t)(m0 + g + 8 * h) * RP + c * 32 + PER * t + 4 * q);
+        hi[c][q][h] = __byte_perm(v[q].x, v[q].y, 0x5410); lo[c][q][h] = __byte_perm(v[q].x, v[q].y, 0x7632);
+        hi[c][q][2 + h] = __byte_perm(v[q].z, v[q].w, 0x5410); lo[c][q][2 + h] = __byte_perm(v[q].z, v[q].w, 0x7632);
+      }
+    }
+  uint32_t now = 0, next = (C::D - 1) * C::STAGE;         // stages that are read and filled
+  uint32_t b_from[4];       // this thread's chunk of each MMA's rows of B (the ring begins at a multiple of 128: chunks 4 further on are 64 bytes apart by a bit)
 #pragma unroll
-          for (int q = 0; q < PER / 4; ++q) {
-            const float4 d = *reinterpret_cast<const float4 *>(w + 4 * q);
-            v[4 * q] += d.x; v[4 * q + 1] += d.y; v[4 * q + 2] += d.z; v[4 * q + 3] += d.w;
+  for (int j = 0; j < 4; ++j) {
+    const int col = column + 8 * (g >> 1) + 2 * j + (g & 1);
+    b_from[j] = base + (RP == 16 ? C::b_at(col, t >> 1) + (t & 1) * 8 : C::b_at(col, t));
+  }
+  T *op0 = o0 + n_first + column + 8 * t, *op1 = o1 + n_first + column + 8 * t;
+#pragma unroll 1
+  for (int i = 0; i < steps; ++i) {
+    stage_wait<C::D - 2>();
+    __syncthreads();
+    if (i + C::D - 1 < steps) fill(next, n_first + (i + C::D - 1) * C::NC);
+    stage_commit();
+#pragma unroll
+    for (int u = 0; u < C::UNITS; ++u) {
+      const int n = n_first + i * C::NC + column + 32 * u;
+      float acc[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[j][q] = 0.0f;
+        // columns of MMA j: g -> n + 8 (g / 2) + 2 j + g % 2, so that this thread's results (columns 2 t, 2 t + 1 of each) are n + 8 t + 2 j, + 1
+        if (RP == 16) {
+          const uint2 w = lds8(b_from[j] + now + u * 32 * C::CH * 16);
+          mma_bf16(acc[j], hi[0][0][0], hi[0][0][1], hi[0][0][2], hi[0][0][3], w.x, w.y);
+          mma_bf16(acc[j], lo[0][0][0], lo[0][0][1], lo[0][0][2], lo[0][0][3], w.x, w.y);
+        } else {
+#pragma unroll
+          for (int c = 0; c < KC; ++c) {
+            const uint4 w = lds16((b_from[j] ^ (C::CH >= 8 ? (c & 1) * 64 : 0)) + (c >> 1) * 128 + now + u * 32 * C::CH * 16);
+            mma_bf16(acc[j], hi[c][0][0], hi[c][0][1], hi[c][0][2], hi[c][0][3], w.x, w.y);
+            mma_bf16(acc[j], lo[c][0][0], lo[c][0][1], lo[c][0][2], lo[c][0][3], w.x, w.y);
+            mma_bf16(acc[j], hi[c][1][0], hi[c][1][1], hi[c][1][2], hi[c][1][3], w.z, w.w);
+            mma_bf16(acc[j], lo[c][1][0], lo[c][1][1], lo[c][1][2], lo[c][1][3], w.z, w.w);
           }
         }
       }
+      const uint32_t y_at = y_to + now + u * 2 * C::Y_UNIT;
 #pragma unroll
-      for (int i = 0; i < PER / 2; ++i) {
-        float a[2], b[2];
+      for (int h = 0; h < 2; ++h) {
+        if (!(h ? live1 : live0)) continue;
+        float f[8];
+        staged_y<T>(y_at + h * C::Y_UNIT, f);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          // (behind the rank: not 0 * infinity, which is what an infinity in x has left there)
-          const float f = c * 32 + PER * t + 2 * i + e < p.R ? __fmul_rn(v[2 * i + e], scale) : 0.0f;
-          a[e] = __bfloat162float(__float2bfloat16_rn(f));
-          b[e] = isfinite(a[e]) ? __fsub_rn(f, a[e]) : 0.0f;        // (exact)
+        for (int j = 0; j < 4; ++j) {
+          f[2 * j] = __fadd_rn(f[2 * j], acc[j][2 * h]);
+          f[2 * j + 1] = __fadd_rn(f[2 * j + 1], acc[j][2 * h + 1]);
         }
-        // pair i -> MMA i / 2, k half i % 2; registers {row g, row g + 8} x {k half}
-        hi[c][i >> 1][2 * (i & 1) + h] = pack_bf16(a[0], a[1]);
-        lo[c][i >> 1][2 * (i & 1) + h] = pack_bf16(b[0], b[1]);
+        if (p.y_vec && i + 1 < steps) Row8<T>::store((h ? op1 : op0) + 32 * u, f);        // (only the last step may pass N)
+        else store_y<T>(h ? o1 : o0, n + 8 * t, p.N, p.y_vec, f);
       }
     }
-  const uint16_t *b = p.b + (int64_t)adapter * p.N * p.R;
-#pragma unroll 1
-  for (int n = n_first; n < n_end; n += NSTEP) {
-    float f0[8] = {}, f1[8] = {};
-    if (live0) load_y<T>(y0, n + 8 * t, p.N, p.y_vec, f0);
-    if (live1) load_y<T>(y1, n + 8 * t, p.N, p.y_vec, f1);
-    float acc[4][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
-      // columns of MMA j: g -> n + 8 (g / 2) + 2 j + g % 2, so that this thread's results (columns 2 t, 2 t + 1 of each) are n + 8 t + 2 j, + 1
-      const int col = n + 8 * (g >> 1) + 2 * j + (g & 1);
-      const uint16_t *row = b + (int64_t)col * p.R;
-      if (RP == 16) {
-        uint2 w = make_uint2(0, 0);
-        if (p.b_vec) {
-          if (col < p.N && 4 * t < p.R) w = __ldg(reinterpret_cast<const uint2 *>(row + 4 * t));
-        } else if (col < p.N) {
-          uint32_t u[2] = {0, 0};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) if (4 * t + i < p.R) u[i >> 1] |= (uint32_t)__ldg(row + 4 * t + i) << (16 * (i & 1));
-          w = make_uint2(u[0], u[1]);
-        }
-        mma_bf16(acc[j], hi[0][0][0], hi[0][0][1], hi[0][0][2], hi[0][0][3], w.x, w.y);
-        mma_bf16(acc[j], lo[0][0][0], lo[0][0][1], lo[0][0][2], lo[0][0][3], w.x, w.y);
-      } else {
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-          const uint4 w = load8<false>(row, c * 32 + 8 * t, col < p.N ? p.R : 0, p.b_vec);
-          mma_bf16(acc[j], hi[c][0][0], hi[c][0][1], hi[c][0][2], hi[c][0][3], w.x, w.y);
-          mma_bf16(acc[j], lo[c][0][0], lo[c][0][1], lo[c][0][2], lo[c][0][3], w.x, w.y);
-          mma_bf16(acc[j], hi[c][1][0], hi[c][1][1], hi[c][1][2], hi[c][1][3], w.z, w.w);
-          mma_bf16(acc[j], lo[c][1][0], lo[c][1][1], lo[c][1][2], lo[c][1][3], w.z, w.w);
-        }
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f0[2 * j] = __fadd_rn(f0[2 * j], acc[j][0]); f0[2 * j + 1] = __fadd_rn(f0[2 * j + 1], acc[j][1]);
-      f1[2 * j] = __fadd_rn(f1[2 * j], acc[j][2]); f1[2 * j + 1] = __fadd_rn(f1[2 * j + 1], acc[j][3]);
-    }
-    if (live0) store_y<T>(o0, n + 8 * t, p.N, p.y_vec, f0);
-    if (live1) store_y<T>(o1, n + 8 * t, p.N, p.y_vec, f1);
+    op0 += C::NC;
+    op1 += C::NC;
+    now = now + C::STAGE == C::D * C::STAGE ? 0 : now + C::STAGE;
+    next = next + C::STAGE == C::D * C::STAGE ? 0 : next + C::STAGE;
   }
 }
 
@@ -347,37 +528,79 @@ struct Plan {
   int64_t tiles;
 };
 
+// bytes of the two kernels' rings (y of 16 bits)
+struct Rings { int shrink, expand; };
+template <int TM>
+static Rings rings_of(int rp) {
+  if (rp == 16) return {Shrink<TM, 16>::SMEM, Expand<TM, 16, __half>::SMEM};
+  if (rp == 32) return {Shrink<TM, 32>::SMEM, Expand<TM, 32, __half>::SMEM};
+  if (rp == 64) return {Shrink<TM, 64>::SMEM, Expand<TM, 64, __half>::SMEM};
+  return {Shrink<TM, 128>::SMEM, Expand<TM, 128, __half>::SMEM};
+}
+
 // How a call is cut, from its sizes alone.  Tiles of 64 rows where a request has 32 or more on average, else of 16.
 static Plan plan_of(int64_t rows, int64_t requests, int64_t K, int64_t N, int64_t R, int sms) {
   Plan pl;
   pl.tm = rows >= 32 * requests ? 64 : 16;
   pl.rp = R <= 16 ? 16 : (R <= 32 ? 32 : (R <= 64 ? 64 : 128));
   pl.tiles = ragged_max_tiles(rows, requests, pl.tm);
-  // tiles with rows: at most the bound less the two of no request
+  // tiles of requests: at most the bound less the two of none
   const int64_t busy = pl.tiles - 2 < rows ? pl.tiles - 2 : rows;
-  // slices of K: blocks enough for four on an SM, each with a loop of 512 k at least
-  const int64_t unit = pl.tm == 64 ? 128 : 512;
-  int64_t slices = ceil_div((int64_t)4 * sms, busy);
-  const int64_t most = ceil_div(K, 512);
-  if (slices > most) slices = most;
-  if (slices > 16) slices = 16;
-  pl.k_slice = (int)align_up(ceil_div(K, slices), unit);
-  pl.slices = (int)ceil_div(K, pl.k_slice);
-  // columns of a block: as many as leave eight blocks for an SM, 128 to 1024
-  int64_t blocks = ceil_div((int64_t)8 * sms, busy);
-  int64_t nb = align_up(ceil_div(N, blocks), 128);
-  if (nb > 1024) nb = 1024;
-  pl.n_block = (int)nb;
+  // One wave of blocks for both kernels: a block of four warps that is alone in a second wave costs as much as the first one.  Blocks that are
+  // resident on an SM go by the shared memory of their rings, at most four.  Slices of K: 1, 2, 4 or 8 blocks of a cluster, of at least 512 k.
+  const Rings rings = pl.tm == 64 ? rings_of<64>(pl.rp) : rings_of<16>(pl.rp);
+  auto wave = [&](int bytes) { return (int64_t)sms * (bytes > 56 * 1024 ? (bytes > 74 * 1024 ? 2 : 3) : 4); };
+  const int64_t unit = pl.tm == 64 ? 64 : 256;
+  pl.slices = 1;
+  while (pl.slices < 8 && busy * pl.slices * 2 <= wave(rings.shrink) && K >= 512 * 2 * pl.slices) pl.slices *= 2;
+  pl.k_slice = (int)align_up(ceil_div(K, pl.slices), unit);
+  // columns of a block: steps of 128
+  const int64_t blocks = busy < wave(rings.expand) ? wave(rings.expand) / busy : 1;
+  pl.n_block = (int)align_up(ceil_div(N, blocks), 128);
   return pl;
+}
+
+template <typename K>
+static int allow_smem(K kern, int bytes, PerDevice<int> &once) {
+  int unused = 0;
+  return once.get(&unused, [&](int &v) {
+    AC4K_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    v = 1;
+    return 0;
+  });
+}
+
+template <int TM, int RP, typename T>
+static int launch_expand(const Args &p, const Plan &pl, cudaStream_t stream) {
+  using C = Expand<TM, RP, T>;
+  static PerDevice<int> once;
+  if (int e = allow_smem(lora_expand_kernel<TM, RP, T>, C::SMEM, once)) return e;
+  return launch_kernel<true>(lora_expand_kernel<TM, RP, T>, dim3((unsigned)pl.tiles, (unsigned)ceil_div(p.N, pl.n_block)), kThreads, C::SMEM, stream, p);
 }
 
 template <int TM, int RP>
 static int launch_rank(const Args &p, const Plan &pl, int dt, cudaStream_t stream) {
-  if (int e = launch_kernel<true>(lora_shrink_kernel<TM, RP>, dim3((unsigned)pl.tiles, (unsigned)pl.slices), kThreads, 0, stream, p)) return e;
-  const dim3 grid((unsigned)pl.tiles, (unsigned)ceil_div(p.N, pl.n_block));
-  if (dt == AC4K_DT_BF16) return launch_kernel<true>(lora_expand_kernel<TM, RP, __nv_bfloat16>, grid, kThreads, 0, stream, p);
-  if (dt == AC4K_DT_FP16) return launch_kernel<true>(lora_expand_kernel<TM, RP, __half>, grid, kThreads, 0, stream, p);
-  return launch_kernel<true>(lora_expand_kernel<TM, RP, float>, grid, kThreads, 0, stream, p);
+  using C = Shrink<TM, RP>;
+  static PerDevice<int> once;
+  if (int e = allow_smem(lora_shrink_kernel<TM, RP>, C::SMEM, once)) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(pl.tiles * pl.slices));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = pl.slices;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pl.slices > 1 ? 2 : 1;
+  AC4K_CUDA_TRY(cudaLaunchKernelEx(&cfg, lora_shrink_kernel<TM, RP>, p));
+  if (dt == AC4K_DT_BF16) return launch_expand<TM, RP, __nv_bfloat16>(p, pl, stream);
+  if (dt == AC4K_DT_FP16) return launch_expand<TM, RP, __half>(p, pl, stream);
+  return launch_expand<TM, RP, float>(p, pl, stream);
 }
 template <int TM>
 static int launch_tm(const Args &p, const Plan &pl, int dt, cudaStream_t stream) {
@@ -409,7 +632,7 @@ extern "C" int ac4k_lora_workspace(int64_t rows, int64_t requests, int64_t K, in
   DeviceInfo di;
   if (int e = get_device_info(&di)) return e;
   const lora::Plan pl = lora::plan_of(rows, requests, K, N, R, di.sms);
-  *bytes = (int64_t)pl.slices * rows * pl.rp * (int64_t)sizeof(float);
+  *bytes = rows * pl.rp * (int64_t)sizeof(uint32_t);
   return 0;
 }
 
@@ -442,22 +665,22 @@ extern "C" int ac4k_lora(void *out, const void *y, int y_dtype, const void *x, c
   DeviceInfo di;
   if (int e = get_device_info(&di)) return e;
   const lora::Plan pl = lora::plan_of(rows, requests, K, N, R, di.sms);
-  if (!workspace || workspace_bytes < (int64_t)pl.slices * rows * pl.rp * (int64_t)sizeof(float))
+  if (!workspace || workspace_bytes < rows * pl.rp * (int64_t)sizeof(uint32_t))
     return fail(AC4K_ERR_SHAPE, "the workspace is smaller than ac4k_lora_workspace says");
   if (addr(workspace) & 15) return fail(AC4K_ERR_ALIGN, "the workspace is not 16-byte aligned");
   lora::Args p = {};
   p.x = static_cast<const uint16_t *>(x); p.a = static_cast<const uint16_t *>(a); p.b = static_cast<const uint16_t *>(b);
   p.y = y; p.out = out;
   p.offsets = offsets; p.adapters = adapters; p.scaling = scaling;
-  p.ws = static_cast<float *>(workspace);
+  p.ws = static_cast<uint32_t *>(workspace);
   p.x_stride = x_stride; p.y_stride = y_stride; p.out_stride = out_stride;
   p.rows = (int)rows; p.requests = (int)requests; p.count = (int)n_adapters;
   p.K = (int)K; p.N = (int)N; p.R = (int)R;
   p.slices = pl.slices; p.k_slice = pl.k_slice; p.n_block = pl.n_block;
-  // 16-byte vectors (b: 8 bytes of a rank up to 16): whole ones in every row, and rows that begin on one
+  // 16-byte vectors: whole ones in every row, and rows that begin on one
   p.x_vec = K % 8 == 0 && x_stride % 8 == 0 && (addr(x) & 15) == 0;
   p.a_vec = K % 8 == 0 && (addr(a) & 15) == 0;
-  p.b_vec = (R % 8 == 0 || (pl.rp == 16 && R % 4 == 0)) && (addr(b) & 15) == 0;
+  p.b_vec = R % 8 == 0 && (addr(b) & 15) == 0;
   const int lanes = 16 / size;
   p.y_vec = N % 8 == 0 && y_stride % lanes == 0 && out_stride % lanes == 0 && ((addr(y) | addr(out)) & 15) == 0;
   if (pl.tm == 64) return lora::launch_tm<64>(p, pl, y_dtype, stream);
