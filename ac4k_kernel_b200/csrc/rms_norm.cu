@@ -39,6 +39,17 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+// two fp32 operations in one instruction, each rounded as the single one is
+__device__ __forceinline__ void add2(float &a, float &b, float c, float d) {
+  asm("{\n.reg .b64 p, q;\nmov.b64 p, {%0, %1};\nmov.b64 q, {%2, %3};\nadd.rn.f32x2 p, p, q;\nmov.b64 {%0, %1}, p;\n}" : "+f"(a), "+f"(b) : "f"(c), "f"(d));
+}
+__device__ __forceinline__ void mul2(float &a, float &b, float c, float d) {
+  asm("{\n.reg .b64 p, q;\nmov.b64 p, {%0, %1};\nmov.b64 q, {%2, %3};\nmul.rn.f32x2 p, p, q;\nmov.b64 {%0, %1}, p;\n}" : "+f"(a), "+f"(b) : "f"(c), "f"(d));
+}
+__device__ __forceinline__ void square_add2(float &a, float &b, float c, float d) {       // a += c * c, b += d * d
+  asm("{\n.reg .b64 p, q;\nmov.b64 p, {%0, %1};\nmov.b64 q, {%2, %3};\nfma.rn.f32x2 p, q, q, p;\nmov.b64 {%0, %1}, p;\n}" : "+f"(a), "+f"(b) : "f"(c), "f"(d));
+}
+
 __device__ __forceinline__ void unpack8(const uint4 &w, float (&f)[8]) {
   const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -59,6 +70,18 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
 __device__ __forceinline__ void load8_f32(const float *p, float (&f)[8]) {
   const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
   f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+}
+
+// 8 weights from column `at` on; ones where there is no weight
+__device__ __forceinline__ void weight8(const Args &p, int at, float (&w)[8]) {
+  if (p.weight == nullptr) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = 1.0f;
+  } else if (p.weight_f32) {
+    load8_f32(static_cast<const float *>(p.weight) + at, w);
+  } else {
+    unpack8(__ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.weight) + at)), w);
+  }
 }
 
 __device__ __forceinline__ float rstd_of(float sum, const Args &p) {
@@ -115,7 +138,7 @@ __device__ __forceinline__ void reduce_row(float &sum, float &amax, float *part)
 
 // Rows of 16-byte vectors: G threads share a row (a warp, or the block), C chunks of 8 elements in registers each.
 template <int FMT, int G, int C, int THREADS>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, C == 8 ? 512 / THREADS : 1)
 rms_norm_kernel(const norm::Args p) {
   using namespace norm;
   static_assert(G == 32 || G == THREADS, "a row per warp or per block");
@@ -130,41 +153,56 @@ rms_norm_kernel(const norm::Args p) {
   }
   const int nfull = (int)(p.K / 8);
   float s[C][8];
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int ch = c * G + t;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (ch < nfull) v = __ldcs(reinterpret_cast<const uint4 *>(p.x + row * p.x_stride + ch * 8));
-    unpack8(v, s[c]);
-  }
-  if (p.residual != nullptr) {
+  if (p.residual != nullptr && !p.residual_f32) {
+    // all loads in front of the first use: x and the residual of the whole row are in flight together
+    const uint16_t *res = static_cast<const uint16_t *>(p.residual) + row * p.residual_stride;
+    uint4 v[C], u[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int ch = c * G + t;
-      float r[8];
+      v[c] = u[c] = make_uint4(0, 0, 0, 0);
       if (ch < nfull) {
-        if (p.residual_f32) {
+        v[c] = __ldcs(reinterpret_cast<const uint4 *>(p.x + row * p.x_stride + ch * 8));
+        u[c] = __ldcs(reinterpret_cast<const uint4 *>(res + ch * 8));
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      float r[8];
+      unpack8(v[c], s[c]);
+      unpack8(u[c], r);
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) add2(s[c][i], s[c][i + 1], r[i], r[i + 1]);
+    }
+  } else {
+    uint4 v[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int ch = c * G + t;
+      v[c] = make_uint4(0, 0, 0, 0);
+      if (ch < nfull) v[c] = __ldcs(reinterpret_cast<const uint4 *>(p.x + row * p.x_stride + ch * 8));
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) unpack8(v[c], s[c]);
+    if (p.residual != nullptr) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int ch = c * G + t;
+        if (ch < nfull) {
           const float4 *q = reinterpret_cast<const float4 *>(static_cast<const float *>(p.residual) + row * p.residual_stride + ch * 8);
           const float4 a = __ldcs(q), b = __ldcs(q + 1);
-          r[0] = a.x; r[1] = a.y; r[2] = a.z; r[3] = a.w; r[4] = b.x; r[5] = b.y; r[6] = b.z; r[7] = b.w;
-        } else unpack8(__ldcs(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.residual) + row * p.residual_stride + ch * 8)), r);
+          const float r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[c][i] = __fadd_rn(s[c][i], r[i]);
+          for (int i = 0; i < 8; ++i) s[c][i] = __fadd_rn(s[c][i], r[i]);
+        }
       }
     }
   }
   grid_launch_dependents();
-  float sum = 0.0f, amax = 0.0f;
-  float w[C][8];
+  float sum = 0.0f, odd = 0.0f, amax = 0.0f;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int ch = c * G + t;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[c][i] = 1.0f;
-    if (p.weight != nullptr && ch < nfull) {
-      if (p.weight_f32) load8_f32(static_cast<const float *>(p.weight) + ch * 8, w[c]);
-      else unpack8(__ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.weight) + ch * 8)), w[c]);
-    }
     if (p.residual_out != nullptr && ch < nfull) {
       if (p.residual_f32) {
         float4 *d = reinterpret_cast<float4 *>(static_cast<float *>(p.residual_out) + row * p.K + ch * 8);
@@ -175,11 +213,18 @@ rms_norm_kernel(const norm::Args p) {
       }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      sum = __fmaf_rn(s[c][i], s[c][i], sum);
-      if (FMT == kE4m3) amax = max_nan(amax, fabsf(__fmul_rn(s[c][i], w[c][i])));
+    for (int i = 0; i < 8; i += 2) square_add2(sum, odd, s[c][i], s[c][i + 1]);
+    if (FMT == kE4m3 && ch < nfull) {
+      float w[8];             // (loaded again behind the reduction: held, they would cost as many registers as the row)
+      weight8(p, ch * 8, w);
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        mul2(w[i], w[i + 1], s[c][i], s[c][i + 1]);
+        amax = max_nan(max_nan(amax, fabsf(w[i])), fabsf(w[i + 1]));
+      }
     }
   }
+  sum = __fadd_rn(sum, odd);
   reduce_row<G>(sum, amax, part);
   const float rstd = rstd_of(sum, p);
   float r = 0.0f, alpha = 0.0f;
@@ -192,12 +237,16 @@ rms_norm_kernel(const norm::Args p) {
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int ch = c * G + t;
-    float v[8];
+    float v[8] = {};
+    if (ch < nfull) {
+      float w[8];
+      weight8(p, ch * 8, w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(__fmul_rn(s[c][i], rstd), w[c][i]);
-    if (ch >= nfull) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+      for (int i = 0; i < 8; i += 2) {
+        v[i] = s[c][i]; v[i + 1] = s[c][i + 1];
+        mul2(v[i], v[i + 1], rstd, rstd);
+        mul2(v[i], v[i + 1], w[i], w[i + 1]);
+      }
     }
     if (FMT == kBf16) {
       if (ch < nfull) *reinterpret_cast<uint4 *>(p.out + (row * p.K + ch * 8) * 2) = pack8(v);
@@ -205,10 +254,10 @@ rms_norm_kernel(const norm::Args p) {
     }
     if (p.normed != nullptr && ch < nfull) *reinterpret_cast<uint4 *>(p.normed + row * p.K + ch * 8) = pack8(v);
     if (FMT == kE4m3) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) mul2(v[i], v[i + 1], r, r);
       if (ch * 8 < Kp)
-        *reinterpret_cast<uint2 *>(p.out + row * Kp + ch * 8) =
-            make_uint2(f32x4_to_e4m3x4(__fmul_rn(v[0], r), __fmul_rn(v[1], r), __fmul_rn(v[2], r), __fmul_rn(v[3], r)),
-                       f32x4_to_e4m3x4(__fmul_rn(v[4], r), __fmul_rn(v[5], r), __fmul_rn(v[6], r), __fmul_rn(v[7], r)));
+        *reinterpret_cast<uint2 *>(p.out + row * Kp + ch * 8) = make_uint2(f32x4_to_e4m3x4(v[0], v[1], v[2], v[3]), f32x4_to_e4m3x4(v[4], v[5], v[6], v[7]));
     }
     if (FMT == kNvfp4) {
       // two neighbouring lanes hold a block of 16, eight a word of four scales (G is a multiple of 8, so they stay in step)
@@ -326,10 +375,19 @@ static int launch_norm_fmt(const norm::Args &p, bool vectors, cudaStream_t strea
   if (Kp <= 512) return launch_norm<FMT, 32, 2, 128>(p, rows, stream);
   if (Kp <= 1024) return launch_norm<FMT, 32, 4, 128>(p, rows, stream);
   if (Kp <= 2048) return launch_norm<FMT, 128, 2, 128>(p, rows, stream);
-  if (Kp <= 4096) return launch_norm<FMT, 256, 2, 256>(p, rows, stream);
-  if (Kp <= 8192) return launch_norm<FMT, 512, 2, 512>(p, rows, stream);
-  if (Kp <= 16384) return launch_norm<FMT, 1024, 2, 1024>(p, rows, stream);
-  return launch_norm<FMT, 1024, 4, 1024>(p, rows, stream);
+  if (rows < 1024) {
+    if (Kp <= 4096) return launch_norm<FMT, 256, 2, 256>(p, rows, stream);
+    if (Kp <= 8192) return launch_norm<FMT, 512, 2, 512>(p, rows, stream);
+    if (Kp <= 16384) return launch_norm<FMT, 1024, 2, 1024>(p, rows, stream);
+    return launch_norm<FMT, 1024, 4, 1024>(p, rows, stream);
+  }
+  if (Kp <= 4096) return launch_norm<FMT, 128, 4, 128>(p, rows, stream);
+  if (Kp <= 5120) return launch_norm<FMT, 128, 5, 128>(p, rows, stream);
+  if (Kp <= 6144) return launch_norm<FMT, 128, 6, 128>(p, rows, stream);
+  if (Kp <= 8192) return launch_norm<FMT, 128, 8, 128>(p, rows, stream);
+  if (Kp <= 12288) return launch_norm<FMT, 256, 6, 256>(p, rows, stream);
+  if (Kp <= 16384) return launch_norm<FMT, 256, 8, 256>(p, rows, stream);
+  return launch_norm<FMT, 512, 8, 512>(p, rows, stream);
 }
 
 }  // namespace ac4k

@@ -113,6 +113,26 @@ def test_against_the_formula(m, k, residual, weight):
 
 
 @gpu
+@pytest.mark.parametrize("k", [2048, 2056, 3000, 4096, 4104, 5120, 5128, 6144, 6152, 8192, 8200, 12288, 12296, 16384, 16392, 20000])
+@pytest.mark.parametrize("residual,weight", [(torch.bfloat16, torch.bfloat16), (None, None), (torch.float32, torch.float32)])
+def test_many_rows(k, residual, weight):
+    """As many rows as take fewer threads each"""
+    from ac4k_kernel_b200 import ops
+    x, w, r = inputs(1030, k, residual, weight, seed=k)
+    s, v = formula(x, w, r, 1e-6)
+    got = ops.rms_norm(x, w, 1e-6, residual=r)
+    out, total = got if r is not None else (got, None)
+    near_bf16(out, v)
+    assert r is None or torch.equal(total, (x.float() + r.float()).to(r.dtype))
+    got = ops.rms_norm(x, w, 1e-6, residual=r, precision="fp8e4m3", keep=True)
+    assert torch.equal(got[2], out) and (r is None or torch.equal(got[3], total))
+    near_fp8(got[0], got[1], v)
+    g = (v.abs().max() / 2688).float()
+    got = ops.rms_norm(x, w, 1e-6, residual=r, precision="nvfp4", global_scale=g, sf_layout="128x4")
+    near_nvfp4(got[0], got[1], g, v, "128x4")
+
+
+@gpu
 @pytest.mark.parametrize("k", [64, 100, 1024, 2048, 4096, 8192, 16384, 32768])
 @pytest.mark.parametrize("precision", [None, "fp8e4m3", "nvfp4"])
 def test_a_row_is_the_same_alone_and_in_a_batch(k, precision):
