@@ -183,8 +183,10 @@ __device__ __forceinline__ void store_out(typename OutT<OUT_DT>::type *dst, floa
 // host helpers (linear_nvfp4.cu)
 // 2-D byte tensor map [rows, row_bytes] with a (128 B x box_rows) box and 128-byte swizzle
 int get_tmap(const void *ptr, int64_t rows, int64_t row_bytes, int box_rows, CUtensorMap *out);
-// the same map made anew
+// the same map made anew, and so for the next two
 int make_tmap(const void *ptr, int64_t rows, int64_t row_bytes, int box_rows, CUtensorMap *out);
+int make_tmap_rows4(const void *ptr, int64_t rows, int64_t row_bytes, CUtensorMap *lo, CUtensorMap *hi);
+int make_tmap_sf_rows(const void *ptr, int64_t rows, int64_t kt, CUtensorMap *out);
 // same bytes with the rows as (row / 4, row % 4): a box of 128 B x 32 x 4 brings rows 4 l + q of a 128-row block to
 // shared-memory row q * 32 + l.  rows no multiple of 4: `lo` has the classes row % 4 < rows % 4 (boxes 128 B x 32 x rows % 4), `hi`
 // the others; else `hi` is left alone
@@ -217,5 +219,11 @@ int launch_linear_2cta(int d_dtype, int sf_mode, const CUtensorMap &ta, const CU
 // decode-shape kernel (linear_nvfp4_skinny.cu): M <= nt activation rows, nt in {16, 32, 64}
 int launch_linear_skinny(int d_dtype, bool sf_tiled, int nt, const CUtensorMap &tx, const CUtensorMap &tw, const GemmArgs &args,
                          cudaStream_t stream);
+
+// products with a weight per group in CTA pairs (linear_nvfp4_grouped_2cta.cu): whether it can take a call, and the call
+bool grouped_pair_takes(int d_dtype, int64_t M, int64_t groups, int64_t N, int64_t K);
+int launch_linear_grouped_pair(void *D, int d_dtype, const void *A, const void *A_sf, const float *A_gs, const void *B, const void *B_sf,
+                               const float *B_gs, int b_gs_stride, const void *bias, int bias_dtype, const int32_t *offsets, bool fill, int64_t M,
+                               int64_t groups, int64_t N, int64_t K, int sms, unsigned int *status, unsigned long long wait_ns, cudaStream_t stream);
 
 }  // namespace ac4k

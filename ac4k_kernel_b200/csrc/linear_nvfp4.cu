@@ -491,6 +491,18 @@ int make_tmap(const void *ptr, int64_t rows, int64_t row_bytes, int box_rows, CU
   return encode(kTmapOperand, ptr, row_bytes, rows, row_bytes, BKB, box_rows, 0, 1, out);
 }
 
+int make_tmap_rows4(const void *ptr, int64_t rows, int64_t row_bytes, CUtensorMap *lo, CUtensorMap *hi) {
+  const int r = rows % 4 ? (int)(rows % 4) : 4;
+  if (int e = encode(kTmapOperand, ptr, row_bytes, rows, row_bytes, BKB, 32, r, r, lo)) return e;
+  if (r == 4) return 0;
+  if (rows < 4) return fail(AC4K_ERR_SHAPE, "fewer than four rows");
+  return encode(kTmapOperand, static_cast<const uint8_t *>(ptr) + r * row_bytes, row_bytes, rows - r, row_bytes, BKB, 32, 4 - r, 4 - r, hi);
+}
+
+int make_tmap_sf_rows(const void *ptr, int64_t rows, int64_t kt, CUtensorMap *out) {
+  return encode(kTmapWords, ptr, rows, kt, rows, 128, 4, 0, 1, out);
+}
+
 // Tiled scale factors [row blocks of 128][K/64][512 bytes] seen as a matrix of 512-byte rows: a box of
 // `box_ksteps` rows is the scale image of that many K steps of one row block, contiguous in shared
 // memory.  Rows past the end of the tensor read as zero.

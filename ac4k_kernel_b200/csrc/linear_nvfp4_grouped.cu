@@ -22,6 +22,7 @@ static constexpr int KS = 4;                     // K = 64 steps per stage (K = 
 static constexpr int W_BYTES = 128 * BKB;        // 128 weight rows x 128 bytes
 static constexpr int SF_BYTES = KS * 512;        // scale chunks of one 128-row block
 static constexpr int kThreads = 192;
+static constexpr int kPairRows = 48;             // groups of more rows than this on average go to the CTA pairs
 template <int NT>
 struct Cfg {
   static constexpr int X_BYTES = NT * BKB;
@@ -409,6 +410,9 @@ extern "C" int ac4k_linear_nvfp4_grouped(void *D, int d_dtype, const void *A, co
 
   const int64_t used = groups < M ? groups : M;        // groups that can have rows
   const int64_t mean = ceil_div(M, used);
+  if (mean > grouped::kPairRows && grouped_pair_takes(d_dtype, M, groups, N, K))
+    return launch_linear_grouped_pair(D, d_dtype, A, A_sf, A_gs, B, B_sf, B_gs, b_gs_per_group ? 1 : 0, bias, bias_dtype, offsets, fill != 0, M, groups, N,
+                                      K, di.sms, status, debug_wait_ns() ? debug_wait_ns() : kWaitTimeoutNs, stream);
   const int nt = mean <= 16 ? 16 : (mean <= 32 ? 32 : (mean <= 64 ? 64 : 128));
   const int64_t tiles_n = ceil_div(N, 128);
   const int64_t tiles = ragged_max_tiles(M, used, nt), busy = tiles - 2 < M ? tiles - 2 : M;

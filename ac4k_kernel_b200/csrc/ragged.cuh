@@ -59,7 +59,7 @@ __device__ __forceinline__ RaggedTile ragged_tile(const int32_t *__restrict__ of
     int lo = bound(e0);
     for (int e = e0; e < e1; ++e) {
       const int hi = bound(e + 1), n = hi > lo ? (hi - lo + tile - 1) / tile : 0;
-      if (want < before + n) {
+      if ((unsigned)(want - before) < (unsigned)n) {        // (within the group whatever the sums of offsets that are none have come to)
         const int r = lo + (want - before) * tile;
         sh->found = RaggedTile{e == 0 || e == entries - 1 ? -1 : e - 1, r, min(r + tile, hi)};
         break;
