@@ -548,12 +548,9 @@ def lora(out, y, x, a, b, offsets, adapters, scaling=None):
     for t in (out, x, a, b, offsets, adapters, scaling):
         _require(t is None or t.device == y.device, "all tensors must be on one device")
     with torch.cuda.device(y.device):
-        need = ctypes.c_int64(0)
-        check(LIB.ac4k_lora_workspace(T, S, K, N, R, ctypes.byref(need)), "lora")
-        ws = torch.empty((need.value // 4,), dtype=torch.float32, device=y.device)
         check(LIB.ac4k_lora(out.data_ptr(), y.data_ptr(), _DT[y.dtype], x.data_ptr(), a.data_ptr(), b.data_ptr(), offsets.data_ptr(),
-                            adapters.data_ptr(), None if scaling is None else scaling.data_ptr(), ws.data_ptr(), need.value, T, S, L, K, N, R,
-                            x.stride(0), y.stride(0), out.stride(0), _stream(y)),
+                            adapters.data_ptr(), None if scaling is None else scaling.data_ptr(), T, S, L, K, N, R, x.stride(0),
+                            y.stride(0), out.stride(0), _stream(y)),
               "lora")
 
 

@@ -56,8 +56,7 @@ SIGNATURES = {
                                    ctypes.c_int64, _vp]),
     "ac4k_rms_norm": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp, _vp, ctypes.c_int, _vp, ctypes.c_int,
                                      ctypes.c_float, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _vp]),
-    "ac4k_lora_workspace": (ctypes.c_int, [ctypes.c_int64] * 5 + [_c_i64p]),
-    "ac4k_lora": (ctypes.c_int, [_vp, _vp, ctypes.c_int] + [_vp] * 7 + [ctypes.c_int64] * 10 + [_vp]),
+    "ac4k_lora": (ctypes.c_int, [_vp, _vp, ctypes.c_int] + [_vp] * 6 + [ctypes.c_int64] * 9 + [_vp]),
     "ac4k_linear_nvfp4_grouped": (ctypes.c_int, [_vp, ctypes.c_int] + [_vp] * 6 + [ctypes.c_int, _vp, ctypes.c_int, _vp, ctypes.c_int] +
                                   [ctypes.c_int64] * 4 + [_vp]),
     "ac4k_peer_alloc": (ctypes.c_int, [ctypes.c_int64, ctypes.POINTER(_vp), ctypes.c_char_p]),

@@ -346,13 +346,10 @@ py::object lora(py::handle hy, py::handle hx, py::handle ha, py::handle hb, py::
   const c10::cuda::CUDAGuard guard(y.device());
   unlocked([&] {
     if (!out.defined()) out = empty({T, N}, y.scalar_type(), y);
-    int64_t bytes = 0;
-    check(ac4k_lora_workspace(T, S, K, N, R, &bytes), "lora");
-    const at::Tensor ws = empty({bytes / 4}, at::kFloat, y);
     check(ac4k_lora(out.data_ptr(), y.data_ptr(), dt_code(y.scalar_type()), x->data_ptr(), a->data_ptr(), b->data_ptr(),
                     static_cast<const int32_t *>(offsets->data_ptr()), static_cast<const int32_t *>(adapters->data_ptr()),
-                    scaling.defined() ? static_cast<const float *>(scaling.data_ptr()) : nullptr, ws.data_ptr(), bytes, T, S, L, K, N, R, x->stride(0),
-                    y.stride(0), out.stride(0), stream_of(y)),
+                    scaling.defined() ? static_cast<const float *>(scaling.data_ptr()) : nullptr, T, S, L, K, N, R, x->stride(0), y.stride(0),
+                    out.stride(0), stream_of(y)),
           "lora");
   });
   return hout.is_none() ? py::cast(out) : py::reinterpret_borrow<py::object>(hout);

@@ -3,17 +3,20 @@
 //   out[t] = y[t] + scaling[a] * B_a (A_a x[t]),   a = adapters[request of row t], or none: out[t] = y[t]
 //
 // A rank of 8 to 128 makes 2 R operations per byte of x and of y, below what the memory allows for up to R = 64: the work is to read x, y and the
-// adapters once and to write out once.  Two launches: `shrink` leaves A x (R values a row), `expand` adds B of it to y.  Both take a
-// tile of rows of one request against its adapter with mma.sync (16 x 8 x 16, bf16, fp32 accumulators): the tiles are small and ragged, no operand
+// adapters once and to write out once.  One launch: a cluster of up to 8 blocks takes a tile of rows of one request.  Each block sums A x over its
+// slice of K ("shrink"), the blocks add their sums in order through distributed shared memory (no atomics, the same result each time), and each
+// adds B of that to its slice of y's columns ("expand").  Nothing goes through global memory in between, and the second half's first operands
+// are on their way while the sums are exchanged.  (As two launches with A x in a workspace: 15.7 us for 64 requests of one token, rank 16,
+// 8192 x 8192; 52 us for 4099 rows, rank 64, 4096 x 4096; 89 us for 8192 rows, rank 32, 8192 x 8192.)
+//
+// Both halves use mma.sync (16 x 8 x 16, bf16, fp32 accumulators): the tiles are small and ragged, no operand
 // is read twice from global memory by a warp, and what tcgen05 would add, rate, is not what bounds them.  Operands come through
 // rings in shared memory (cp.async), x and y each thread's own 16-byte vectors, the adapter's shared by the block: a product's sum may run
 // over k in any order, so a thread takes 8 neighbouring k of a row and deals them to the two MMAs of a step of 32 k, the same for both
-// operands, and needs no ldmatrix; the columns of `expand` are dealt so that the 8 results
+// operands, and needs no ldmatrix; the columns of the second half are dealt so that the 8 results
 // of a thread over four MMAs are neighbours, which it loads from y and stores in vectors.
 //
-// A x is summed in fp32 and handed over as two bf16 values (16 bits of mantissa together), for which `expand` takes two MMAs.
-// K is cut into slices where there are few tiles; the slices of a tile are a cluster, which adds their sums in order: no atomics, the same result
-// each time, and `expand` reads 4 bytes a value (it read every slice's sums at first: 137 MB through L2 for 4099 rows of rank 64 in 7 slices).
+// A x is summed in fp32 and handed over as two bf16 values (16 bits of mantissa together), for which the second half takes two MMAs.
 #include "ragged.cuh"
 #include "sm100_ptx.cuh"
 
@@ -23,18 +26,22 @@ namespace lora {
 static constexpr int kThreads = 128;      // four warps
 static constexpr int kMaxRank = 128;
 
+// Blocks that an SM's 228 KB take (1 KB each is the system's, and the block has some hundred bytes more)
+constexpr int blocks_of(int bytes) { return bytes <= 55 * 1024 ? 4 : (bytes <= 74 * 1024 ? 3 : (bytes <= 111 * 1024 ? 2 : 1)); }
+// Stages of a ring: as many as leave room for four blocks on an SM; for the adapters of high ranks three or two
+constexpr int stages_of(int tm, int rp, int stage) { return (rp <= 32 || (tm == 64 && rp == 64) ? 54 : (rp == 64 || tm == 64 ? 73 : 110)) * 1024 / stage; }
+
 struct Args {
   const uint16_t *x, *a, *b;   // x [rows, K], a [adapters, R, K], b [adapters, N, R]
   const void *y;
   void *out;
   const int32_t *offsets, *adapters;
   const float *scaling;        // or NULL: ones
-  uint32_t *ws;                // [rows][RP]: scaling * A x, a bf16 value (low half) and what it leaves of the fp32 one
   int64_t x_stride, y_stride, out_stride;
   int rows, requests, count;   // count: adapters
   int K, N, R;
-  int slices, k_slice;         // K of a slice, a multiple of the step of a warp's loop
-  int n_block;                 // columns of a block of `expand`
+  int slices;                  // blocks of a cluster
+  int k_slice, n_slice;        // K and columns of a block, multiples of a stage's
   bool x_vec, a_vec, b_vec, y_vec;
 };
 
@@ -88,167 +95,6 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 }  // namespace lora
-
-namespace lora {
-// `shrink`: what a stage of the ring holds.  KW: k of a warp in a stage; TM 64: all warps the same k, TM 16: in turn.
-template <int TM, int RP>
-struct Shrink {
-  static constexpr int KW = TM == 64 || RP <= 32 ? 64 : 32;
-  static constexpr int KB = TM == 64 ? KW : 4 * KW;             // k of the block
-  static constexpr int PARTS = KB / KW;
-  static constexpr int CH = KW / 8;                             // 16-byte chunks of a row
-  static constexpr int X_BYTES = kThreads * (KW / 32) * 2 * 16; // each thread its own two rows' chunks
-  static constexpr int A_PART = RP * KW * 2;
-  static constexpr int STAGE = X_BYTES + PARTS * A_PART;
-  static constexpr int D = TM == 64 ? 4 : (RP == 128 || RP == 32 ? 3 : 4);
-  static constexpr int SMEM = D * STAGE;
-  // chunk c of adapter row r: rows of 8 chunks lie with their halves exchanged in every other row, so that the eight threads of a phase
-  // (two rows, four chunks) meet all banks; two rows of 4 chunks do by themselves
-  static __device__ __forceinline__ uint32_t a_at(int r, int c) { return (uint32_t)(r * CH + (CH == 8 ? c ^ ((r & 1) << 2) : c)) * 16u; }
-};
-}  // namespace lora
-
-// A x: a block takes one tile of rows and one slice of K.  TM 64: a warp per 16 rows, all of the slice; TM 16 (a few rows a request): the
-// warps divide each stage's k, and the block adds their sums.  The adapter's rows are shared by the block, x by nobody: a
-// thread loads just what it feeds to its MMAs.
-template <int TM, int RP>
-__global__ void __launch_bounds__(lora::kThreads)
-lora_shrink_kernel(const lora::Args p) {
-  using namespace lora;
-  using C = Shrink<TM, RP>;
-  constexpr int NT = RP / 8;
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ RaggedScratch scratch;
-  grid_dependency_wait();
-  grid_launch_dependents();
-  const int slice = p.slices > 1 ? (int)ptx::cluster_ctarank() : 0;
-  const RaggedTile tile = ragged_tile<kThreads>(p.offsets, p.requests, p.rows, TM, blockIdx.x / p.slices, &scratch);
-  if (tile.group < 0) return;               // (the blocks of a cluster have the same tile)
-  const int adapter = adapter_of(p, tile);
-  if (adapter < 0) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int m0 = tile.row0 + (TM == 64 ? warp * 16 : 0), r0 = m0 + g, r1 = m0 + g + 8;
-  const int k0 = min(p.K, slice * p.k_slice), k1 = min(p.K, k0 + p.k_slice);
-  const bool live0 = r0 < tile.row1, live1 = r1 < tile.row1;
-  const uint16_t *x0 = p.x + (int64_t)(live0 ? r0 : tile.row0) * p.x_stride, *x1 = p.x + (int64_t)(live1 ? r1 : tile.row0) * p.x_stride;
-  const uint16_t *a = p.a + (int64_t)adapter * p.R * p.K;
-  const uint32_t base = shared_addr(smem);
-  const int part = TM == 64 ? 0 : warp;
-  float acc[NT][4];
-#pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
-  // A stage, from k on.  In whole vectors a thread has its places worked out once: its two rows of x, and of the adapter one row in every ROWS, which
-  // move on by a stage's k each time (worked out anew for each load, a stage of rank 32 took 294 instructions a warp, 16 of them MMAs: 50 us
-  // for 8192 x 8192, and the memory idle two thirds of the time).
-  constexpr int LOADS = RP * C::CH * C::PARTS / kThreads, ROWS = kThreads / C::CH;
-  static_assert(RP % ROWS == 0, "a thread's loads lie in one column of chunks");
-  const int a_c = threadIdx.x % C::CH, a_r = threadIdx.x / C::CH;
-  const uint16_t *xp0 = x0 + k0 + part * C::KW + 8 * t, *xp1 = x1 + k0 + part * C::KW + 8 * t;
-  const uint16_t *ap = a + (int64_t)a_r * p.K + k0 + a_c * 8;
-  const int64_t a_rows = (int64_t)ROWS * p.K;
-  const uint32_t x_to = base + threadIdx.x * 16, a_to = base + C::X_BYTES + C::a_at(a_r, a_c);
-  const uint32_t bytes0 = live0 ? 16 : 0, bytes1 = live1 ? 16 : 0;
-  auto fill = [&](uint32_t off, int k) {
-    if (p.x_vec && p.a_vec && k + C::KB <= k1) {
-#pragma unroll
-      for (int u = 0; u < C::KW / 32; ++u) {
-        stage16(x_to + off + (2 * u) * kThreads * 16, xp0 + u * 32, bytes0);
-        stage16(x_to + off + (2 * u + 1) * kThreads * 16, xp1 + u * 32, bytes1);
-      }
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int r = i * ROWS % RP, q = i * ROWS / RP;
-        stage16(a_to + off + q * C::A_PART + r * C::CH * 16, ap + (r / ROWS) * a_rows + q * C::KW, a_r + r < p.R ? 16 : 0);
-      }
-      xp0 += C::KB;
-      xp1 += C::KB;
-      ap += C::KB;
-      return;
-    }
-#pragma unroll
-    for (int u = 0; u < C::KW / 32; ++u) {
-      const int kk = k + part * C::KW + u * 32 + 8 * t;
-      stage8(x_to + off + (2 * u) * kThreads * 16, x0, kk, live0 ? k1 : 0, p.x_vec);
-      stage8(x_to + off + (2 * u + 1) * kThreads * 16, x1, kk, live1 ? k1 : 0, p.x_vec);
-    }
-#pragma unroll 1
-    for (int i = threadIdx.x; i < RP * C::CH * C::PARTS; i += kThreads) {
-      const int q = i / (RP * C::CH), r = i / C::CH % RP, c = i % C::CH;
-      stage8(base + off + C::X_BYTES + q * C::A_PART + C::a_at(r, c), a + (int64_t)(r < p.R ? r : 0) * p.K, k + q * C::KW + c * 8, r < p.R ? k1 : 0, p.a_vec);
-    }
-  };
-  const int steps = (k1 - k0 + C::KB - 1) / C::KB;
-#pragma unroll
-  for (int i = 0; i < C::D - 1; ++i) {
-    if (i < steps) fill(i * C::STAGE, k0 + i * C::KB);
-    stage_commit();
-  }
-  uint32_t now = 0, next = (C::D - 1) * C::STAGE;         // stages that are read and filled
-  const uint32_t x_at = base + threadIdx.x * 16, a_at0 = base + C::X_BYTES + part * C::A_PART + C::a_at(g, t);
-  const uint32_t a_at1 = base + C::X_BYTES + part * C::A_PART + C::a_at(g, C::CH == 8 ? 4 + t : t);
-#pragma unroll 1
-  for (int i = 0; i < steps; ++i) {
-    stage_wait<C::D - 2>();
-    __syncthreads();              // stage i is there for all, and all are done with the one that is filled next
-    if (i + C::D - 1 < steps) fill(next, k0 + (i + C::D - 1) * C::KB);
-    stage_commit();
-#pragma unroll
-    for (int u = 0; u < C::KW / 32; ++u) {
-      const uint4 xa = lds16(x_at + now + (2 * u) * kThreads * 16), xb = lds16(x_at + now + (2 * u + 1) * kThreads * 16);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const uint4 w = lds16((u ? a_at1 : a_at0) + now + j * 8 * C::CH * 16);
-        mma_bf16(acc[j], xa.x, xb.x, xa.y, xb.y, w.x, w.y);
-        mma_bf16(acc[j], xa.z, xb.z, xa.w, xb.w, w.z, w.w);
-      }
-    }
-    now = now + C::STAGE == C::D * C::STAGE ? 0 : now + C::STAGE;
-    next = next + C::STAGE == C::D * C::STAGE ? 0 : next + C::STAGE;
-  }
-  // The sums of this block's slice, [row of the tile][RP], then those of all slices: the blocks of the cluster take a share of the values each, add
-  // them in the order of the slices, scale and round them to two bf16 parts.
-  float *sums = reinterpret_cast<float *>(smem);
-  constexpr int WARPS = TM == 64 ? 1 : 4;               // sums of a row
-  static_assert(WARPS * TM * RP * 4 <= C::SMEM, "the sums reuse the ring");
-  stage_wait<0>();
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    float *d = sums + (warp * 16 + g) * RP + 8 * j + 2 * t;
-    *reinterpret_cast<float2 *>(d) = make_float2(acc[j][0], acc[j][1]);
-    *reinterpret_cast<float2 *>(d + 8 * RP) = make_float2(acc[j][2], acc[j][3]);
-  }
-  if (p.slices > 1) ptx::cluster_sync();
-  else __syncthreads();
-  const float scale = p.scaling != nullptr ? __ldg(p.scaling + adapter) : 1.0f;
-  const int n = (tile.row1 - tile.row0) * RP;
-  uint32_t *ws = p.ws + (int64_t)tile.row0 * RP;
-  for (int i = (slice * kThreads + threadIdx.x) * 4; i < n; i += p.slices * kThreads * 4) {
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int q = 0; q < p.slices; ++q) {
-      const uint32_t at = p.slices > 1 ? ptx::map_to_cta(base + i * 4, q) : base + i * 4;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        float4 d;
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(d.x), "=f"(d.y), "=f"(d.z), "=f"(d.w) : "r"(at + w * 16 * RP * 4) : "memory");
-        v.x += d.x; v.y += d.y; v.z += d.z; v.w += d.w;
-      }
-    }
-    const float f[4] = {v.x, v.y, v.z, v.w};
-    uint32_t u[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      // (behind the rank: not 0 * infinity, which is what an infinity in x has left there)
-      const float a = i % RP + e < p.R ? __fmul_rn(f[e], scale) : 0.0f;
-      const float h = __bfloat162float(__float2bfloat16_rn(a));
-      u[e] = pack_bf16(h, isfinite(h) ? __fsub_rn(a, h) : 0.0f);        // (the difference is exact)
-    }
-    *reinterpret_cast<uint4 *>(ws + i) = make_uint4(u[0], u[1], u[2], u[3]);
-  }
-  if (p.slices > 1) ptx::cluster_sync();                // no block leaves while another still reads its sums
-}
 
 namespace lora {
 template <typename T> struct Row8;      // 8 neighbouring values of y
@@ -347,17 +193,39 @@ __device__ __forceinline__ void store_y(T *row, int n, int N, bool vec, const fl
 }  // namespace lora
 
 namespace lora {
-// `expand`: what a stage of the ring holds: the rows of B of NC columns, and y's values for each thread's results
+// What a stage of the first half's ring holds.  KW: k of a warp in a stage; TM 64: all warps the same k, TM 16: in turn.
+template <int TM, int RP>
+struct Shrink {
+  static constexpr int KW = (TM == 64 && RP <= 64) || RP <= 16 ? 64 : 32;
+  static constexpr int KB = TM == 64 ? KW : 4 * KW;             // k of the block
+  static constexpr int PARTS = KB / KW;
+  static constexpr int CH = KW / 8;                             // 16-byte chunks of a row
+  static constexpr int X_BYTES = kThreads * (KW / 32) * 2 * 16; // each thread its own two rows' chunks
+  static constexpr int A_PART = RP * KW * 2;
+  static constexpr int STAGE = X_BYTES + PARTS * A_PART;
+  static constexpr int D = stages_of(TM, RP, STAGE);
+  // chunk c of adapter row r: rows of 8 chunks lie with their halves exchanged in every other row, so that the eight threads of a phase
+  // (two rows, four chunks) meet all banks; two rows of 4 chunks do by themselves
+  static __device__ __forceinline__ uint32_t a_at(int r, int c) { return (uint32_t)(r * CH + (CH == 8 ? c ^ ((r & 1) << 2) : c)) * 16u; }
+};
+// What a stage of the second half's ring holds: the rows of B of NC columns, and y's values for each thread's results
 template <int TM, int RP, typename T>
 struct Expand {
-  static constexpr int UNITS = TM == 64 ? 2 : 1;                // of 32 columns, for each warp
-  static constexpr int NC = TM == 64 ? 64 : 128;
+  static constexpr int UNITS = TM == 64 && (RP == 16 || (RP == 32 && sizeof(T) == 2)) ? 2 : 1;      // of 32 columns, for each warp
+  static constexpr int NC = (TM == 64 ? 32 : 128) * UNITS;
   static constexpr int CH = RP / 8;
   static constexpr int B_BYTES = NC * RP * 2;
   static constexpr int Y_UNIT = kThreads * (int)sizeof(T) * 8;  // one row's values of a unit
   static constexpr int STAGE = B_BYTES + UNITS * 2 * Y_UNIT;
-  static constexpr int D = RP == 128 ? 3 : 4;
-  static constexpr int SMEM = D * STAGE;
+  // In front of the first stage that may be filled while the sums are exchanged: the block's own sums, and the total in two parts
+  static constexpr int SUMS = (TM == 64 ? 1 : 4) * TM * RP * 4, PARTS2 = TM * RP * 4;
+  static constexpr int FIRST = (SUMS + PARTS2 + STAGE - 1) / STAGE;
+  static constexpr int D0 = stages_of(TM, RP, STAGE);
+  static constexpr int D = D0 > FIRST ? D0 : FIRST;
+  static constexpr int EARLY = D - FIRST < D - 1 ? D - FIRST : D - 1;             // stages filled that early
+  static constexpr int SMEM = D * STAGE > Shrink<TM, RP>::D * Shrink<TM, RP>::STAGE ? D * STAGE : Shrink<TM, RP>::D * Shrink<TM, RP>::STAGE;
+  static constexpr int BLOCKS = blocks_of(SMEM);                // on an SM
+  static_assert(D >= 2 && Shrink<TM, RP>::D >= 2 && SMEM + 2048 <= 227 * 1024, "a ring has two stages");
   // chunk c of B's row n.  The eight threads of a phase read four chunks of rows n, n + 1: as in Shrink.  Rank 16: sixteen threads read halves
   // of chunks of rows n, n + 1, n + 8, n + 9; pairs of rows change places in every other eight.
   static __device__ __forceinline__ uint32_t b_at(int n, int c) {
@@ -367,84 +235,219 @@ struct Expand {
 };
 }  // namespace lora
 
-// y + B (A x): a block takes one tile of rows and n_block columns, a warp 16 rows and 32 columns at a time.  TM 64: the warps have 16 rows each,
-// the same columns; TM 16: the same rows, columns in turn.
+// A block takes one tile of rows, one slice of K and one of the columns.  TM 64: a warp per 16 rows; TM 16 (a few rows a request): the warps divide
+// each stage's k and add their sums, then its columns.  The adapter's rows are shared by the block, x and y by nobody: a
+// thread loads just what it feeds to its MMAs and what it adds to its results.
 template <int TM, int RP, typename T>
-__global__ void __launch_bounds__(lora::kThreads)
-lora_expand_kernel(const lora::Args p) {
+__global__ void __launch_bounds__(lora::kThreads, lora::Expand<TM, RP, T>::BLOCKS)
+lora_kernel(const lora::Args p) {
   using namespace lora;
-  using C = Expand<TM, RP, T>;
-  constexpr int KC = RP / 32 > 0 ? RP / 32 : 1;      // steps of 32 k (one of 16 for rank 16)
+  using S1 = Shrink<TM, RP>;
+  using S2 = Expand<TM, RP, T>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ RaggedScratch scratch;
-  // The offsets, y and the adapters may be read in front of the wait: the shrink kernel's blocks let this one in behind their own wait, so
-  // all that was enqueued before them is complete.
-  const RaggedTile tile = ragged_tile<kThreads>(p.offsets, p.requests, p.rows, TM, blockIdx.x, &scratch);
-  const int adapter = tile.group == -2 ? -1 : adapter_of(p, tile);
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int slice = p.slices > 1 ? (int)ptx::cluster_ctarank() : 0;
+  const RaggedTile tile = ragged_tile<kThreads>(p.offsets, p.requests, p.rows, TM, blockIdx.x / p.slices, &scratch);
+  if (tile.group == -2) return;             // (the blocks of a cluster have the same tile)
+  const int adapter = adapter_of(p, tile);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int n_first = blockIdx.y * p.n_block, n_end = min(p.N, n_first + p.n_block);
-  const int m0 = tile.row0 + (TM == 64 ? warp * 16 : 0), column = TM == 64 ? 0 : warp * 32;
-  const bool live0 = tile.group != -2 && m0 + g < tile.row1, live1 = tile.group != -2 && m0 + g + 8 < tile.row1;
-  const T *y0 = static_cast<const T *>(p.y) + (int64_t)(m0 + g) * p.y_stride, *y1 = y0 + 8 * p.y_stride;
-  T *o0 = static_cast<T *>(p.out) + (int64_t)(m0 + g) * p.out_stride, *o1 = o0 + 8 * p.out_stride;
-  if (tile.group == -2 || adapter < 0) {
-    grid_dependency_wait();
-    grid_launch_dependents();
-    if (tile.group == -2 || p.out == p.y) return;
+  const int m0 = tile.row0 + (TM == 64 ? warp * 16 : 0), r0 = m0 + g, r1 = m0 + g + 8;
+  const bool live0 = r0 < tile.row1, live1 = r1 < tile.row1;
+  const int n_first = min(p.N, slice * p.n_slice), n_end = min(p.N, n_first + p.n_slice), column = TM == 64 ? 0 : warp * 32;
+  const T *y0 = static_cast<const T *>(p.y) + (int64_t)r0 * p.y_stride, *y1 = y0 + 8 * p.y_stride;
+  T *o0 = static_cast<T *>(p.out) + (int64_t)r0 * p.out_stride, *o1 = o0 + 8 * p.out_stride;
+  if (adapter < 0) {
+    if (p.out == p.y) return;
     for (int n = n_first + column; n < n_end; n += TM == 64 ? 32 : 128) {     // rows without an adapter
       if (live0) copy8<T>(o0, y0, n + 8 * t, p.N, p.y_vec);
       if (live1) copy8<T>(o1, y1, n + 8 * t, p.N, p.y_vec);
     }
     return;
   }
-  const uint16_t *b = p.b + (int64_t)adapter * p.N * p.R;
   const uint32_t base = shared_addr(smem);
+  if (TM == 16 && p.b_vec && n_first < n_end)      // the block's rows of B, read by no other tile: on their way to L2 from the start
+    ptx::bulk_prefetch_l2_if(threadIdx.x == 0, p.b + ((int64_t)adapter * p.N + n_first) * p.R, (uint32_t)min((n_end - n_first) * p.R * 2ll, 65536ll));
+  {
+    // ------------------------------------------------------------------ A x over the block's k
+    constexpr int NT = RP / 8;
+    const int k0 = min(p.K, slice * p.k_slice), k1 = min(p.K, k0 + p.k_slice);
+    const uint16_t *x0 = p.x + (int64_t)(live0 ? r0 : tile.row0) * p.x_stride, *x1 = p.x + (int64_t)(live1 ? r1 : tile.row0) * p.x_stride;
+    const uint16_t *a = p.a + (int64_t)adapter * p.R * p.K;
+    const int part = TM == 64 ? 0 : warp;
+    float acc[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
+    // A stage, from k on.  In whole vectors a thread has its places worked out once: its two rows of x, and of the adapter one row in every ROWS, which
+    // move on by a stage's k each time (worked out anew for each load, a stage of rank 32 took 294 instructions a warp, 16 of them MMAs: 50 us
+    // for 8192 x 8192, and the memory idle two thirds of the time).
+    constexpr int LOADS = RP * S1::CH * S1::PARTS / kThreads, ROWS = kThreads / S1::CH;
+    static_assert(RP % ROWS == 0, "a thread's loads lie in one column of chunks");
+    const int a_c = threadIdx.x % S1::CH, a_r = threadIdx.x / S1::CH;
+    const uint16_t *xp0 = x0 + k0 + part * S1::KW + 8 * t, *xp1 = x1 + k0 + part * S1::KW + 8 * t;
+    const uint16_t *ap = a + (int64_t)a_r * p.K + k0 + a_c * 8;
+    const int64_t a_rows = (int64_t)ROWS * p.K;
+    const uint32_t x_to = base + threadIdx.x * 16, a_to = base + S1::X_BYTES + S1::a_at(a_r, a_c);
+    const uint32_t bytes0 = live0 ? 16 : 0, bytes1 = live1 ? 16 : 0;
+    auto fill = [&](uint32_t off, int k) {
+      if (p.x_vec && p.a_vec && k + S1::KB <= k1) {
+#pragma unroll
+        for (int u = 0; u < S1::KW / 32; ++u) {
+          stage16(x_to + off + (2 * u) * kThreads * 16, xp0 + u * 32, bytes0);
+          stage16(x_to + off + (2 * u + 1) * kThreads * 16, xp1 + u * 32, bytes1);
+        }
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+          const int r = i * ROWS % RP, q = i * ROWS / RP;
+          stage16(a_to + off + q * S1::A_PART + r * S1::CH * 16, ap + (r / ROWS) * a_rows + q * S1::KW, a_r + r < p.R ? 16 : 0);
+        }
+        xp0 += S1::KB;
+        xp1 += S1::KB;
+        ap += S1::KB;
+        return;
+      }
+#pragma unroll
+      for (int u = 0; u < S1::KW / 32; ++u) {
+        const int kk = k + part * S1::KW + u * 32 + 8 * t;
+        stage8(x_to + off + (2 * u) * kThreads * 16, x0, kk, live0 ? k1 : 0, p.x_vec);
+        stage8(x_to + off + (2 * u + 1) * kThreads * 16, x1, kk, live1 ? k1 : 0, p.x_vec);
+      }
+#pragma unroll 1
+      for (int i = threadIdx.x; i < RP * S1::CH * S1::PARTS; i += kThreads) {
+        const int q = i / (RP * S1::CH), r = i / S1::CH % RP, c = i % S1::CH;
+        stage8(base + off + S1::X_BYTES + q * S1::A_PART + S1::a_at(r, c), a + (int64_t)(r < p.R ? r : 0) * p.K, k + q * S1::KW + c * 8, r < p.R ? k1 : 0, p.a_vec);
+      }
+    };
+    const int steps = (k1 - k0 + S1::KB - 1) / S1::KB;
+#pragma unroll
+    for (int i = 0; i < S1::D - 1; ++i) {
+      if (i < steps) fill(i * S1::STAGE, k0 + i * S1::KB);
+      stage_commit();
+    }
+    uint32_t now = 0, next = (S1::D - 1) * S1::STAGE;         // stages that are read and filled
+    const uint32_t x_at = base + threadIdx.x * 16, a_at0 = base + S1::X_BYTES + part * S1::A_PART + S1::a_at(g, t);
+    const uint32_t a_at1 = base + S1::X_BYTES + part * S1::A_PART + S1::a_at(g, S1::CH == 8 ? 4 + t : t);
+#pragma unroll 1
+    for (int i = 0; i < steps; ++i) {
+      stage_wait<S1::D - 2>();
+      __syncthreads();              // stage i is there for all, and all are done with the one that is filled next
+      if (i + S1::D - 1 < steps) fill(next, k0 + (i + S1::D - 1) * S1::KB);
+      stage_commit();
+#pragma unroll
+      for (int u = 0; u < S1::KW / 32; ++u) {
+        const uint4 xa = lds16(x_at + now + (2 * u) * kThreads * 16), xb = lds16(x_at + now + (2 * u + 1) * kThreads * 16);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const uint4 w = lds16((u ? a_at1 : a_at0) + now + j * 8 * S1::CH * 16);
+          mma_bf16(acc[j], xa.x, xb.x, xa.y, xb.y, w.x, w.y);
+          mma_bf16(acc[j], xa.z, xb.z, xa.w, xb.w, w.z, w.w);
+        }
+      }
+      now = now + S1::STAGE == S1::D * S1::STAGE ? 0 : now + S1::STAGE;
+      next = next + S1::STAGE == S1::D * S1::STAGE ? 0 : next + S1::STAGE;
+    }
+    // the sums of this slice: [row of the tile][RP], one such array a warp where the warps divide k
+    stage_wait<0>();
+    __syncthreads();
+    float *sums = reinterpret_cast<float *>(smem);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      float *d = sums + (warp * 16 + g) * RP + 8 * j + 2 * t;
+      *reinterpret_cast<float2 *>(d) = make_float2(acc[j][0], acc[j][1]);
+      *reinterpret_cast<float2 *>(d + 8 * RP) = make_float2(acc[j][2], acc[j][3]);
+    }
+  }
+  // ------------------------------------------------------------------ the ring of the second half, and what may be loaded already
+  const uint16_t *b = p.b + (int64_t)adapter * p.N * p.R;
   // A stage, from column n on; whole vectors of whole columns as in `shrink`
-  constexpr int LOADS = C::NC * C::CH / kThreads, COLS = kThreads / C::CH;
-  const int b_c = threadIdx.x % C::CH, b_n = threadIdx.x / C::CH;
+  constexpr int LOADS = S2::NC * S2::CH / kThreads, COLS = kThreads / S2::CH;
+  static_assert(S2::NC % COLS == 0, "every thread has its part of a stage");
+  const int b_c = threadIdx.x % S2::CH, b_n = threadIdx.x / S2::CH;
   const uint16_t *bp = b + (int64_t)(n_first + b_n) * p.R + b_c * 8;
-  const int64_t b_cols = (int64_t)COLS * p.R, b_step = (int64_t)C::NC * p.R;
+  const int64_t b_cols = (int64_t)COLS * p.R, b_step = (int64_t)S2::NC * p.R;
   const T *yp0 = y0 + n_first + column + 8 * t, *yp1 = y1 + n_first + column + 8 * t;
-  const uint32_t b_to = base + C::b_at(b_n, b_c), y_to = base + C::B_BYTES + threadIdx.x * 16, b_bytes = b_c * 8 < p.R ? 16 : 0;
+  const uint32_t b_to = base + S2::b_at(b_n, b_c), y_to = base + S2::B_BYTES + threadIdx.x * 16, b_bytes = b_c * 8 < p.R ? 16 : 0;
   auto fill = [&](uint32_t off, int n) {
-    if (p.b_vec && p.y_vec && n + C::NC <= p.N) {
+    if (p.b_vec && p.y_vec && n + S2::NC <= p.N) {
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) stage16(b_to + off + i * COLS * C::CH * 16, bp + i * b_cols, b_bytes);
+      for (int i = 0; i < LOADS; ++i) stage16(b_to + off + i * COLS * S2::CH * 16, bp + i * b_cols, b_bytes);
 #pragma unroll
-      for (int u = 0; u < C::UNITS; ++u)
+      for (int u = 0; u < S2::UNITS; ++u)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           if (h ? live1 : live0) {
 #pragma unroll
             for (int q = 0; q < (int)sizeof(T) / 2; ++q)
-              stage16(y_to + off + (2 * u + h) * C::Y_UNIT + q * kThreads * 16, (h ? yp1 : yp0) + 32 * u + q * (16 / (int)sizeof(T)), 16);
+              stage16(y_to + off + (2 * u + h) * S2::Y_UNIT + q * kThreads * 16, (h ? yp1 : yp0) + 32 * u + q * (16 / (int)sizeof(T)), 16);
           }
       bp += b_step;
-      yp0 += C::NC;
-      yp1 += C::NC;
+      yp0 += S2::NC;
+      yp1 += S2::NC;
       return;
     }
 #pragma unroll 1
-    for (int i = threadIdx.x; i < C::NC * C::CH; i += kThreads) {
-      const int col = i / C::CH, c = i % C::CH;
+    for (int i = threadIdx.x; i < S2::NC * S2::CH; i += kThreads) {
+      const int col = i / S2::CH, c = i % S2::CH;
       const bool in = n + col < p.N;
-      stage8(base + off + C::b_at(col, c), b + (int64_t)(in ? n + col : 0) * p.R, c * 8, in ? p.R : 0, p.b_vec);
+      stage8(base + off + S2::b_at(col, c), b + (int64_t)(in ? n + col : 0) * p.R, c * 8, in ? p.R : 0, p.b_vec);
     }
 #pragma unroll
-    for (int u = 0; u < C::UNITS; ++u) {
+    for (int u = 0; u < S2::UNITS; ++u) {
       const int col = n + column + 32 * u + 8 * t;
-      stage_y<T>(y_to + off + 2 * u * C::Y_UNIT, y0, col, p.N, live0, p.y_vec);
-      stage_y<T>(y_to + off + (2 * u + 1) * C::Y_UNIT, y1, col, p.N, live1, p.y_vec);
+      stage_y<T>(y_to + off + 2 * u * S2::Y_UNIT, y0, col, p.N, live0, p.y_vec);
+      stage_y<T>(y_to + off + (2 * u + 1) * S2::Y_UNIT, y1, col, p.N, live1, p.y_vec);
     }
   };
-  const int steps = (n_end - n_first + C::NC - 1) / C::NC;
+  const int steps = (n_end - n_first + S2::NC - 1) / S2::NC;
+  constexpr int kFrom = S2::D - S2::EARLY;             // where the first stage lies: those in front of it hold the sums
 #pragma unroll
-  for (int i = 0; i < C::D - 1; ++i) {
-    if (i < steps) fill(i * C::STAGE, n_first + i * C::NC);
+  for (int i = 0; i < S2::EARLY; ++i) {
+    if (i < steps) fill((kFrom + i) * S2::STAGE, n_first + i * S2::NC);
     stage_commit();
   }
-  grid_dependency_wait();
-  grid_launch_dependents();
+  // ------------------------------------------------------------------ the sums of all slices
+  // The blocks of the cluster take a share of the values each, add them in the order of the slices, scale and round them to two bf16 parts (a value
+  // in the low half of a word, what it leaves in the high one) and write them to every block.
+  const uint32_t total = base + S2::SUMS;
+  {
+    constexpr int WARPS = TM == 64 ? 1 : 4;               // sums of a row
+    if (p.slices > 1) ptx::cluster_sync();
+    else __syncthreads();
+    const float scale = p.scaling != nullptr ? __ldg(p.scaling + adapter) : 1.0f;
+    const int n = (tile.row1 - tile.row0) * RP;
+    for (int i = (slice * kThreads + threadIdx.x) * 4; i < n; i += p.slices * kThreads * 4) {
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int q = 0; q < p.slices; ++q) {
+        const uint32_t at = p.slices > 1 ? ptx::map_to_cta(base + i * 4, q) : base + i * 4;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          float4 d;
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(d.x), "=f"(d.y), "=f"(d.z), "=f"(d.w) : "r"(at + w * 16 * RP * 4) : "memory");
+          v.x += d.x; v.y += d.y; v.z += d.z; v.w += d.w;
+        }
+      }
+      const float f[4] = {v.x, v.y, v.z, v.w};
+      uint32_t u[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        // (behind the rank: not 0 * infinity, which is what an infinity in x has left there)
+        const float a = i % RP + e < p.R ? __fmul_rn(f[e], scale) : 0.0f;
+        const float h = __bfloat162float(__float2bfloat16_rn(a));
+        u[e] = pack_bf16(h, isfinite(h) ? __fsub_rn(a, h) : 0.0f);        // (the difference is exact)
+      }
+      for (int q = 0; q < p.slices; ++q) {
+        const uint32_t at = p.slices > 1 ? ptx::map_to_cta(total + i * 4, q) : total + i * 4;
+        asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
+      }
+    }
+    if (p.slices > 1) ptx::cluster_sync();              // behind this no block touches another's memory
+    else __syncthreads();
+  }
+  // ------------------------------------------------------------------ y + B of the sum over the block's columns
+  constexpr int KC = RP / 32 > 0 ? RP / 32 : 1;      // steps of 32 k (one of 16 for rank 16)
   // Both parts of A x for this warp's rows: the fragments of a step of 32 k hold k = 8 t + {0, 1}, {2, 3} (first MMA) and {4, 5}, {6, 7} (second);
   // rank 16: k = 4 t + {0, 1}, {2, 3}.  Pair i -> MMA i / 2, k half i % 2; registers {row g, row g + 8} x {k half}
   uint32_t hi[KC][2][4], lo[KC][2][4];
@@ -457,28 +460,34 @@ lora_expand_kernel(const lora::Args p) {
 #pragma unroll
       for (int q = 0; q < PER / 4; ++q) {
         v[q] = make_uint4(0, 0, 0, 0);
-        if (h ? live1 : live0) v[q] = *reinterpret_cast<const uint4 *>(p.ws + (int64_t)(m0 + g + 8 * h) * RP + c * 32 + PER * t + 4 * q);
+        if (h ? live1 : live0) v[q] = lds16(total + (uint32_t)((r0 - tile.row0 + 8 * h) * RP + c * 32 + PER * t + 4 * q) * 4u);
         hi[c][q][h] = __byte_perm(v[q].x, v[q].y, 0x5410); lo[c][q][h] = __byte_perm(v[q].x, v[q].y, 0x7632);
         hi[c][q][2 + h] = __byte_perm(v[q].z, v[q].w, 0x5410); lo[c][q][2 + h] = __byte_perm(v[q].z, v[q].w, 0x7632);
       }
     }
-  uint32_t now = 0, next = (C::D - 1) * C::STAGE;         // stages that are read and filled
+  __syncthreads();              // all have read the sums: their place is the ring's now
+#pragma unroll
+  for (int i = S2::EARLY; i < S2::D - 1; ++i) {
+    if (i < steps) fill((kFrom + i) % S2::D * S2::STAGE, n_first + i * S2::NC);
+    stage_commit();
+  }
+  uint32_t now = kFrom % S2::D * S2::STAGE, next = (kFrom + S2::D - 1) % S2::D * S2::STAGE;
   uint32_t b_from[4];       // this thread's chunk of each MMA's rows of B (the ring begins at a multiple of 128: chunks 4 further on are 64 bytes apart by a bit)
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int col = column + 8 * (g >> 1) + 2 * j + (g & 1);
-    b_from[j] = base + (RP == 16 ? C::b_at(col, t >> 1) + (t & 1) * 8 : C::b_at(col, t));
+    b_from[j] = base + (RP == 16 ? S2::b_at(col, t >> 1) + (t & 1) * 8 : S2::b_at(col, t));
   }
   T *op0 = o0 + n_first + column + 8 * t, *op1 = o1 + n_first + column + 8 * t;
 #pragma unroll 1
   for (int i = 0; i < steps; ++i) {
-    stage_wait<C::D - 2>();
+    stage_wait<S2::D - 2>();
     __syncthreads();
-    if (i + C::D - 1 < steps) fill(next, n_first + (i + C::D - 1) * C::NC);
+    if (i + S2::D - 1 < steps) fill(next, n_first + (i + S2::D - 1) * S2::NC);
     stage_commit();
 #pragma unroll
-    for (int u = 0; u < C::UNITS; ++u) {
-      const int n = n_first + i * C::NC + column + 32 * u;
+    for (int u = 0; u < S2::UNITS; ++u) {
+      const int n = n_first + i * S2::NC + column + 32 * u;
       float acc[4][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -486,13 +495,13 @@ lora_expand_kernel(const lora::Args p) {
         for (int q = 0; q < 4; ++q) acc[j][q] = 0.0f;
         // columns of MMA j: g -> n + 8 (g / 2) + 2 j + g % 2, so that this thread's results (columns 2 t, 2 t + 1 of each) are n + 8 t + 2 j, + 1
         if (RP == 16) {
-          const uint2 w = lds8(b_from[j] + now + u * 32 * C::CH * 16);
+          const uint2 w = lds8(b_from[j] + now + u * 32 * S2::CH * 16);
           mma_bf16(acc[j], hi[0][0][0], hi[0][0][1], hi[0][0][2], hi[0][0][3], w.x, w.y);
           mma_bf16(acc[j], lo[0][0][0], lo[0][0][1], lo[0][0][2], lo[0][0][3], w.x, w.y);
         } else {
 #pragma unroll
           for (int c = 0; c < KC; ++c) {
-            const uint4 w = lds16((b_from[j] ^ (C::CH >= 8 ? (c & 1) * 64 : 0)) + (c >> 1) * 128 + now + u * 32 * C::CH * 16);
+            const uint4 w = lds16((b_from[j] ^ (S2::CH >= 8 ? (c & 1) * 64 : 0)) + (c >> 1) * 128 + now + u * 32 * S2::CH * 16);
             mma_bf16(acc[j], hi[c][0][0], hi[c][0][1], hi[c][0][2], hi[c][0][3], w.x, w.y);
             mma_bf16(acc[j], lo[c][0][0], lo[c][0][1], lo[c][0][2], lo[c][0][3], w.x, w.y);
             mma_bf16(acc[j], hi[c][1][0], hi[c][1][1], hi[c][1][2], hi[c][1][3], w.z, w.w);
@@ -500,12 +509,12 @@ lora_expand_kernel(const lora::Args p) {
           }
         }
       }
-      const uint32_t y_at = y_to + now + u * 2 * C::Y_UNIT;
+      const uint32_t y_at = y_to + now + u * 2 * S2::Y_UNIT;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         if (!(h ? live1 : live0)) continue;
         float f[8];
-        staged_y<T>(y_at + h * C::Y_UNIT, f);
+        staged_y<T>(y_at + h * S2::Y_UNIT, f);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           f[2 * j] = __fadd_rn(f[2 * j], acc[j][2 * h]);
@@ -515,74 +524,46 @@ lora_expand_kernel(const lora::Args p) {
         else store_y<T>(h ? o1 : o0, n + 8 * t, p.N, p.y_vec, f);
       }
     }
-    op0 += C::NC;
-    op1 += C::NC;
-    now = now + C::STAGE == C::D * C::STAGE ? 0 : now + C::STAGE;
-    next = next + C::STAGE == C::D * C::STAGE ? 0 : next + C::STAGE;
+    op0 += S2::NC;
+    op1 += S2::NC;
+    now = now + S2::STAGE == S2::D * S2::STAGE ? 0 : now + S2::STAGE;
+    next = next + S2::STAGE == S2::D * S2::STAGE ? 0 : next + S2::STAGE;
   }
 }
 
 namespace lora {
 struct Plan {
-  int tm, rp, slices, k_slice, n_block;
+  int slices, k_slice, n_slice;
   int64_t tiles;
 };
 
-// bytes of the two kernels' rings (y of 16 bits)
-struct Rings { int shrink, expand; };
-template <int TM>
-static Rings rings_of(int rp) {
-  if (rp == 16) return {Shrink<TM, 16>::SMEM, Expand<TM, 16, __half>::SMEM};
-  if (rp == 32) return {Shrink<TM, 32>::SMEM, Expand<TM, 32, __half>::SMEM};
-  if (rp == 64) return {Shrink<TM, 64>::SMEM, Expand<TM, 64, __half>::SMEM};
-  return {Shrink<TM, 128>::SMEM, Expand<TM, 128, __half>::SMEM};
-}
-
-// How a call is cut, from its sizes alone.  Tiles of 64 rows where a request has 32 or more on average, else of 16.
-static Plan plan_of(int64_t rows, int64_t requests, int64_t K, int64_t N, int64_t R, int sms) {
+// How a call is cut, from its sizes alone: slices of K and of the columns, 1, 2, 4 or 8 blocks of a cluster, as many as keep the grid in one wave (a
+// block that is alone in a second wave costs as much as the first one) and 512 of K and N together in a block.
+static Plan plan_of(int64_t rows, int64_t requests, int64_t K, int64_t N, int tm, int kb, int nc, int64_t wave) {
   Plan pl;
-  pl.tm = rows >= 32 * requests ? 64 : 16;
-  pl.rp = R <= 16 ? 16 : (R <= 32 ? 32 : (R <= 64 ? 64 : 128));
-  pl.tiles = ragged_max_tiles(rows, requests, pl.tm);
-  // tiles of requests: at most the bound less the two of none
-  const int64_t busy = pl.tiles - 2 < rows ? pl.tiles - 2 : rows;
-  // One wave of blocks for both kernels: a block of four warps that is alone in a second wave costs as much as the first one.  Blocks that are
-  // resident on an SM go by the shared memory of their rings, at most four.  Slices of K: 1, 2, 4 or 8 blocks of a cluster, of at least 512 k.
-  const Rings rings = pl.tm == 64 ? rings_of<64>(pl.rp) : rings_of<16>(pl.rp);
-  auto wave = [&](int bytes) { return (int64_t)sms * (bytes > 56 * 1024 ? (bytes > 74 * 1024 ? 2 : 3) : 4); };
-  const int64_t unit = pl.tm == 64 ? 64 : 256;
+  pl.tiles = ragged_max_tiles(rows, requests, tm);
+  const int64_t busy = pl.tiles - 2 < rows ? pl.tiles - 2 : rows;        // tiles of requests: at most the bound less the two of none
   pl.slices = 1;
-  while (pl.slices < 8 && busy * pl.slices * 2 <= wave(rings.shrink) && K >= 512 * 2 * pl.slices) pl.slices *= 2;
-  pl.k_slice = (int)align_up(ceil_div(K, pl.slices), unit);
-  // columns of a block: steps of 128
-  const int64_t blocks = busy < wave(rings.expand) ? wave(rings.expand) / busy : 1;
-  pl.n_block = (int)align_up(ceil_div(N, blocks), 128);
+  while (pl.slices < 8 && busy * pl.slices * 2 <= wave && K + N >= 1024 * pl.slices) pl.slices *= 2;
+  pl.k_slice = (int)align_up(ceil_div(K, pl.slices), kb);
+  pl.n_slice = (int)align_up(ceil_div(N, pl.slices), nc);
   return pl;
 }
 
-template <typename K>
-static int allow_smem(K kern, int bytes, PerDevice<int> &once) {
-  int unused = 0;
-  return once.get(&unused, [&](int &v) {
-    AC4K_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    v = 1;
-    return 0;
-  });
-}
-
 template <int TM, int RP, typename T>
-static int launch_expand(const Args &p, const Plan &pl, cudaStream_t stream) {
+static int launch_lora(Args p, int sms, cudaStream_t stream) {
   using C = Expand<TM, RP, T>;
+  auto kern = lora_kernel<TM, RP, T>;
   static PerDevice<int> once;
-  if (int e = allow_smem(lora_expand_kernel<TM, RP, T>, C::SMEM, once)) return e;
-  return launch_kernel<true>(lora_expand_kernel<TM, RP, T>, dim3((unsigned)pl.tiles, (unsigned)ceil_div(p.N, pl.n_block)), kThreads, C::SMEM, stream, p);
-}
-
-template <int TM, int RP>
-static int launch_rank(const Args &p, const Plan &pl, int dt, cudaStream_t stream) {
-  using C = Shrink<TM, RP>;
-  static PerDevice<int> once;
-  if (int e = allow_smem(lora_shrink_kernel<TM, RP>, C::SMEM, once)) return e;
+  int unused = 0;
+  if (int e = once.get(&unused, [&](int &v) {
+        AC4K_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        v = 1;
+        return 0;
+      }))
+    return e;
+  const Plan pl = plan_of(p.rows, p.requests, p.K, p.N, TM, Shrink<TM, RP>::KB, C::NC, (int64_t)sms * C::BLOCKS);
+  p.slices = pl.slices; p.k_slice = pl.k_slice; p.n_slice = pl.n_slice;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(pl.tiles * pl.slices));
   cfg.blockDim = dim3(kThreads);
@@ -597,19 +578,30 @@ static int launch_rank(const Args &p, const Plan &pl, int dt, cudaStream_t strea
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pl.slices > 1 ? 2 : 1;
-  AC4K_CUDA_TRY(cudaLaunchKernelEx(&cfg, lora_shrink_kernel<TM, RP>, p));
-  if (dt == AC4K_DT_BF16) return launch_expand<TM, RP, __nv_bfloat16>(p, pl, stream);
-  if (dt == AC4K_DT_FP16) return launch_expand<TM, RP, __half>(p, pl, stream);
-  return launch_expand<TM, RP, float>(p, pl, stream);
+  AC4K_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p));
+  return 0;
+}
+
+template <int TM, int RP>
+static int launch_dtype(const Args &p, int dt, int sms, cudaStream_t stream) {
+  if (dt == AC4K_DT_BF16) return launch_lora<TM, RP, __nv_bfloat16>(p, sms, stream);
+  if (dt == AC4K_DT_FP16) return launch_lora<TM, RP, __half>(p, sms, stream);
+  return launch_lora<TM, RP, float>(p, sms, stream);
 }
 template <int TM>
-static int launch_tm(const Args &p, const Plan &pl, int dt, cudaStream_t stream) {
-  switch (pl.rp) {
-    case 16: return launch_rank<TM, 16>(p, pl, dt, stream);
-    case 32: return launch_rank<TM, 32>(p, pl, dt, stream);
-    case 64: return launch_rank<TM, 64>(p, pl, dt, stream);
-    default: return launch_rank<TM, 128>(p, pl, dt, stream);
-  }
+static int launch_tm(const Args &p, int dt, int sms, cudaStream_t stream) {
+  if (p.R <= 16) return launch_dtype<TM, 16>(p, dt, sms, stream);
+  if (p.R <= 32) return launch_dtype<TM, 32>(p, dt, sms, stream);
+  if (p.R <= 64) return launch_dtype<TM, 64>(p, dt, sms, stream);
+  return launch_dtype<TM, 128>(p, dt, sms, stream);
+}
+
+// Whether two sets of rows share a byte (strides and lengths in bytes).  Rows of one stride may lie between each other.
+static bool rows_overlap(uintptr_t a, int64_t a_stride, int64_t a_len, uintptr_t b, int64_t b_stride, int64_t b_len, int64_t rows) {
+  if (a >= b + (rows - 1) * b_stride + b_len || b >= a + (rows - 1) * a_stride + a_len) return false;
+  if (rows == 1 || a_stride != b_stride || a_stride == 0) return true;
+  const int64_t d = (int64_t)(b - a) % a_stride, behind = d < 0 ? d + a_stride : d;       // where b's rows begin behind a's
+  return behind < a_len || behind + b_len > a_stride;
 }
 
 static int check_sizes(int64_t rows, int64_t requests, int64_t adapters, int64_t K, int64_t N, int64_t R) {
@@ -623,22 +615,9 @@ static int check_sizes(int64_t rows, int64_t requests, int64_t adapters, int64_t
 
 }  // namespace ac4k
 
-extern "C" int ac4k_lora_workspace(int64_t rows, int64_t requests, int64_t K, int64_t N, int64_t R, int64_t *bytes) {
-  using namespace ac4k;
-  if (!bytes) return fail(AC4K_ERR_NULL, "bytes is NULL");
-  *bytes = 0;
-  if (int e = lora::check_sizes(rows, requests, 0, K, N, R)) return e;
-  if (rows == 0 || requests == 0 || K == 0 || N == 0 || R == 0) return 0;
-  DeviceInfo di;
-  if (int e = get_device_info(&di)) return e;
-  const lora::Plan pl = lora::plan_of(rows, requests, K, N, R, di.sms);
-  *bytes = rows * pl.rp * (int64_t)sizeof(uint32_t);
-  return 0;
-}
-
 extern "C" int ac4k_lora(void *out, const void *y, int y_dtype, const void *x, const void *a, const void *b, const int32_t *offsets,
-                         const int32_t *adapters, const float *scaling, void *workspace, int64_t workspace_bytes, int64_t rows, int64_t requests,
-                         int64_t n_adapters, int64_t K, int64_t N, int64_t R, int64_t x_stride, int64_t y_stride, int64_t out_stride,
+                         const int32_t *adapters, const float *scaling, int64_t rows, int64_t requests, int64_t n_adapters,
+                         int64_t K, int64_t N, int64_t R, int64_t x_stride, int64_t y_stride, int64_t out_stride,
                          ac4k_stream_t stream_) {
   using namespace ac4k;
   if (y_dtype < 0 || y_dtype > 2) return fail(AC4K_ERR_ENUM, "unknown y_dtype %d", y_dtype);
@@ -650,8 +629,7 @@ extern "C" int ac4k_lora(void *out, const void *y, int y_dtype, const void *x, c
   const int size = y_dtype == AC4K_DT_FP32 ? 4 : 2;
   auto addr = [](const void *q) { return reinterpret_cast<uintptr_t>(q); };
   if ((addr(y) | addr(out)) & (size - 1)) return fail(AC4K_ERR_ALIGN, "y or out is not aligned to its elements");
-  const uintptr_t y_end = addr(y) + ((rows - 1) * y_stride + N) * size, o_end = addr(out) + ((rows - 1) * out_stride + N) * size;
-  if (out == y ? out_stride != y_stride : (addr(out) < y_end && addr(y) < o_end))
+  if (out == y ? out_stride != y_stride : lora::rows_overlap(addr(out), out_stride * size, N * size, addr(y), y_stride * size, N * size, rows))
     return fail(AC4K_ERR_SHAPE, "out is y itself or does not overlap it");
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   if (n_adapters == 0 || requests == 0 || K == 0 || R == 0) {       // no adapter adds anything
@@ -662,27 +640,24 @@ extern "C" int ac4k_lora(void *out, const void *y, int y_dtype, const void *x, c
   }
   if (!x || !a || !b || !offsets || !adapters) return fail(AC4K_ERR_NULL, "a required pointer is NULL");
   if (((addr(x) | addr(a) | addr(b)) & 1) || ((addr(offsets) | addr(adapters) | addr(scaling)) & 3)) return fail(AC4K_ERR_ALIGN, "a pointer is not aligned to its elements");
+  // (the columns of a row are written while other blocks still read their x)
+  if (lora::rows_overlap(addr(out), out_stride * size, N * size, addr(x), x_stride * 2, K * 2, rows)) return fail(AC4K_ERR_SHAPE, "out overlaps x");
   DeviceInfo di;
   if (int e = get_device_info(&di)) return e;
-  const lora::Plan pl = lora::plan_of(rows, requests, K, N, R, di.sms);
-  if (!workspace || workspace_bytes < rows * pl.rp * (int64_t)sizeof(uint32_t))
-    return fail(AC4K_ERR_SHAPE, "the workspace is smaller than ac4k_lora_workspace says");
-  if (addr(workspace) & 15) return fail(AC4K_ERR_ALIGN, "the workspace is not 16-byte aligned");
   lora::Args p = {};
   p.x = static_cast<const uint16_t *>(x); p.a = static_cast<const uint16_t *>(a); p.b = static_cast<const uint16_t *>(b);
   p.y = y; p.out = out;
   p.offsets = offsets; p.adapters = adapters; p.scaling = scaling;
-  p.ws = static_cast<uint32_t *>(workspace);
   p.x_stride = x_stride; p.y_stride = y_stride; p.out_stride = out_stride;
   p.rows = (int)rows; p.requests = (int)requests; p.count = (int)n_adapters;
   p.K = (int)K; p.N = (int)N; p.R = (int)R;
-  p.slices = pl.slices; p.k_slice = pl.k_slice; p.n_block = pl.n_block;
   // 16-byte vectors: whole ones in every row, and rows that begin on one
   p.x_vec = K % 8 == 0 && x_stride % 8 == 0 && (addr(x) & 15) == 0;
   p.a_vec = K % 8 == 0 && (addr(a) & 15) == 0;
   p.b_vec = R % 8 == 0 && (addr(b) & 15) == 0;
   const int lanes = 16 / size;
   p.y_vec = N % 8 == 0 && y_stride % lanes == 0 && out_stride % lanes == 0 && ((addr(y) | addr(out)) & 15) == 0;
-  if (pl.tm == 64) return lora::launch_tm<64>(p, pl, y_dtype, stream);
-  return lora::launch_tm<16>(p, pl, y_dtype, stream);
+  // tiles of 64 rows where a request has 32 or more on average, else of 16
+  if (rows >= 32 * requests) return lora::launch_tm<64>(p, y_dtype, di.sms, stream);
+  return lora::launch_tm<16>(p, y_dtype, di.sms, stream);
 }

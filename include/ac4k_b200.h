@@ -278,13 +278,10 @@ int ac4k_rms_norm(void *out, void *sf, const float *global_scale, int precision,
  *   stride) or overlaps it nowhere.  a: bf16 [n_adapters, R, K], b: bf16 [n_adapters, N, R], dense; an adapter of a lower rank has zeros
  *   behind it.  offsets: int32 [requests + 1], ascending within [0, rows]; adapters: int32 [requests]; scaling: fp32 [n_adapters] or NULL
  *   (ones); all on the device.  R <= 128.
- * A x is held in fp32 and its product with B in fp32 with 16 bits of each value of A x; one rounding to out.
- * workspace: as many bytes as ac4k_lora_workspace says for the current device, 16-byte aligned, for this call alone (contents undefined). */
-int ac4k_lora_workspace(int64_t rows, int64_t requests, int64_t K, int64_t N, int64_t R, int64_t *bytes);
+ * out does not overlap x either.  A x is held in fp32 and its product with B in fp32 with 16 bits of each value of A x; one rounding to out. */
 int ac4k_lora(void *out, const void *y, int y_dtype, const void *x, const void *a, const void *b, const int32_t *offsets,
-              const int32_t *adapters, const float *scaling, void *workspace, int64_t workspace_bytes, int64_t rows, int64_t requests,
-              int64_t n_adapters, int64_t K, int64_t N, int64_t R, int64_t x_stride, int64_t y_stride, int64_t out_stride,
-              ac4k_stream_t stream);
+              const int32_t *adapters, const float *scaling, int64_t rows, int64_t requests, int64_t n_adapters, int64_t K, int64_t N,
+              int64_t R, int64_t x_stride, int64_t y_stride, int64_t out_stride, ac4k_stream_t stream);
 
 /* ac4k_linear_nvfp4 with a weight per group of rows, e.g. the experts of a layer on rows that are sorted by expert (no counterpart in the
  * reference): for the rows t of group e, [offsets[e], offsets[e + 1]),

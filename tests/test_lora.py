@@ -171,7 +171,7 @@ def test_same_result_each_time_streams_and_graphs():
         side.synchronize()
         assert torch.equal(other, want_d)
     graphs = []
-    for args in (c, d):             # two graphs with workspaces of their own, replayed side by side
+    for args in (c, d):             # two graphs replayed side by side
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             out = ops.lora(*args)
@@ -222,6 +222,9 @@ def test_native_host_side_and_wrapper_agree(monkeypatch):
              dict(out=torch.zeros(26, 48, dtype=torch.bfloat16, device="cuda")[1:, :].as_strided((25, 48), (24, 1)))]
     whole = torch.zeros(26, 48, dtype=torch.bfloat16, device="cuda")
     wrong.append(dict(y=whole[:25], out=whole[1:]))              # overlaps y and is not y
+    both = torch.zeros(25, 128, dtype=torch.bfloat16, device="cuda")
+    wrong.append(dict(x=both[:, :64], out=both[:, 40:88]))       # overlaps x
+    calls.append(dict(x=both[:, :64], out=both[:, 64:112]))      # lies between x's rows
     for number, kw in enumerate(calls + wrong):
         res = []
         for path in (host_calls, None):
@@ -241,16 +244,15 @@ def test_refusals_of_the_c_interface():
     from ac4k_kernel_b200._lib import LIB, last_error
     P = 1 << 20
 
-    def call(out=P, y=2 * P, dt=0, x=P, a=P, b=P, offsets=P, adapters=P, scaling=None, ws=P, wsb=1 << 30, t=4, s=1, l=1, k=64, n=64, r=8, xs=64, ys=64,
+    def call(out=P, y=2 * P, dt=0, x=3 * P, a=P, b=P, offsets=P, adapters=P, scaling=None, t=4, s=1, l=1, k=64, n=64, r=8, xs=64, ys=64,
              os=64):
-        return LIB.ac4k_lora(out, y, dt, x, a, b, offsets, adapters, scaling, ws, wsb, t, s, l, k, n, r, xs, ys, os, None)
+        return LIB.ac4k_lora(out, y, dt, x, a, b, offsets, adapters, scaling, t, s, l, k, n, r, xs, ys, os, None)
 
     for kw, code in ((dict(dt=3), -4), (dict(t=-1), -2), (dict(r=129), -5), (dict(n=1 << 23), -2), (dict(xs=-1), -2), (dict(out=None), -1),
-                     (dict(y=None), -1), (dict(y=2 * P + 1), -3), (dict(y=P + 64), -2), (dict(y=P, ys=128), -2), (dict(os=32), -2),
+                     (dict(y=None), -1), (dict(y=2 * P + 1), -3), (dict(y=P + 64), -2), (dict(x=P + 64), -2), (dict(y=P, ys=128), -2), (dict(os=32), -2),
                      (dict(x=None), -1), (dict(offsets=None), -1), (dict(x=P + 1), -3), (dict(adapters=P + 2), -3), (dict(scaling=P + 1), -3),
                      (dict(l=0, ys=8), -2)):
         assert call(**kw) == code, kw
         assert last_error()
     assert call(t=0, out=None) == 0 and call(n=0) == 0
     assert call(out=P, y=P, l=0, x=None) == 0            # in place and nothing to add
-    assert LIB.ac4k_lora_workspace(4, 1, 64, 64, 8, None) == -1
