@@ -25,6 +25,7 @@ namespace ac4k {
 namespace lora {
 static constexpr int kThreads = 128;      // four warps
 static constexpr int kMaxRank = 128;
+static constexpr int kMaxSlices = 8;      // blocks of a cluster
 
 // Blocks that an SM's 228 KB take (1 KB each is the system's, and the block has some hundred bytes more)
 constexpr int blocks_of(int bytes) { return bytes <= 55 * 1024 ? 4 : (bytes <= 74 * 1024 ? 3 : (bytes <= 111 * 1024 ? 2 : 1)); }
@@ -537,14 +538,18 @@ struct Plan {
   int64_t tiles;
 };
 
-// How a call is cut, from its sizes alone: slices of K and of the columns, 1, 2, 4 or 8 blocks of a cluster, as many as keep the grid in one wave (a
-// block that is alone in a second wave costs as much as the first one) and 512 of K and N together in a block.
-static Plan plan_of(int64_t rows, int64_t requests, int64_t K, int64_t N, int tm, int kb, int nc, int64_t wave) {
+// Blocks that are resident at once, by the size of their clusters (a cluster's blocks share a GPC, whose SMs it need not fill)
+struct Waves { int of[kMaxSlices + 1]; };
+
+// How a call is cut, from its sizes and the device alone: slices of K and of the columns, as many blocks of a cluster as keep the grid in one wave (75
+// tiles of rank 64 in clusters of 8, four more than there was room for, took 42 us, in clusters of 7 38 us) and 512 of K and N together in a block.
+static Plan plan_of(int64_t rows, int64_t requests, int64_t K, int64_t N, int tm, int kb, int nc, const Waves &waves) {
   Plan pl;
   pl.tiles = ragged_max_tiles(rows, requests, tm);
   const int64_t busy = pl.tiles - 2 < rows ? pl.tiles - 2 : rows;        // tiles of requests: at most the bound less the two of none
   pl.slices = 1;
-  while (pl.slices < 8 && busy * pl.slices * 2 <= wave && K + N >= 1024 * pl.slices) pl.slices *= 2;
+  for (int s = 2; s <= kMaxSlices; ++s)
+    if (busy * s <= waves.of[s] && K + N >= 512 * s) pl.slices = s;
   pl.k_slice = (int)align_up(ceil_div(K, pl.slices), kb);
   pl.n_slice = (int)align_up(ceil_div(N, pl.slices), nc);
   return pl;
@@ -554,30 +559,38 @@ template <int TM, int RP, typename T>
 static int launch_lora(Args p, int sms, cudaStream_t stream) {
   using C = Expand<TM, RP, T>;
   auto kern = lora_kernel<TM, RP, T>;
-  static PerDevice<int> once;
-  int unused = 0;
-  if (int e = once.get(&unused, [&](int &v) {
-        AC4K_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-        v = 1;
-        return 0;
-      }))
-    return e;
-  const Plan pl = plan_of(p.rows, p.requests, p.K, p.N, TM, Shrink<TM, RP>::KB, C::NC, (int64_t)sms * C::BLOCKS);
-  p.slices = pl.slices; p.k_slice = pl.k_slice; p.n_slice = pl.n_slice;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(pl.tiles * pl.slices));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = pl.slices;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pl.slices > 1 ? 2 : 1;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  // once per device: the shared-memory attribute, and how many clusters of each size can be resident at once
+  static PerDevice<Waves> once;
+  Waves waves;
+  if (int e = once.get(&waves, [&](Waves &v) {
+        AC4K_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        cfg.numAttrs = 1;
+        for (int s = 2; s <= kMaxSlices; ++s) {
+          int n = 0;
+          cfg.gridDim = dim3((unsigned)(sms * C::BLOCKS / s * s));
+          attr[0].val.clusterDim.x = s;
+          AC4K_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+          v.of[s] = n * s;
+        }
+        return 0;
+      }))
+    return e;
+  const Plan pl = plan_of(p.rows, p.requests, p.K, p.N, TM, Shrink<TM, RP>::KB, C::NC, waves);
+  p.slices = pl.slices; p.k_slice = pl.k_slice; p.n_slice = pl.n_slice;
+  cfg.gridDim = dim3((unsigned)(pl.tiles * pl.slices));
+  attr[0].val.clusterDim.x = pl.slices;
+  cfg.numAttrs = 2;
   AC4K_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p));
   return 0;
 }
