@@ -3,7 +3,7 @@
 //   out[t] = y[t] + scaling[a] * B_a (A_a x[t]),   a = adapters[request of row t], or none: out[t] = y[t]
 //
 // A rank of 8 to 128 makes 2 R operations per byte of x and of y, below what the memory allows for up to R = 64: the work is to read x, y and the
-// adapters once and to write out once.  One launch: a cluster of up to 8 blocks takes a tile of rows of one request.  Each block sums A x over its
+// adapters once and to write out once.  One launch: a cluster of up to 16 blocks takes a tile of rows of one request.  Each block sums A x over its
 // slice of K ("shrink"), the blocks add their sums in order through distributed shared memory (no atomics, the same result each time), and each
 // adds B of that to its slice of y's columns ("expand").  Nothing goes through global memory in between, and the second half's first operands
 // are on their way while the sums are exchanged.  (As two launches with A x in a workspace: 15.7 us for 64 requests of one token, rank 16,
@@ -25,7 +25,7 @@ namespace ac4k {
 namespace lora {
 static constexpr int kThreads = 128;      // four warps
 static constexpr int kMaxRank = 128;
-static constexpr int kMaxSlices = 8;      // blocks of a cluster
+static constexpr int kMaxSlices = 16;     // blocks of a cluster
 
 // Blocks that an SM's 228 KB take (1 KB each is the system's, and the block has some hundred bytes more)
 constexpr int blocks_of(int bytes) { return bytes <= 55 * 1024 ? 4 : (bytes <= 74 * 1024 ? 3 : (bytes <= 111 * 1024 ? 2 : 1)); }
@@ -170,16 +170,37 @@ __device__ __forceinline__ void staged_y(uint32_t src, float (&f)[8]) {
   for (int i = 0; i < PARTS; ++i) v[i] = lds16(src + i * kThreads * 16);
   Row8<T>::load(v, f);
 }
-// the same values bit for bit
+// Columns n, n + step, ... of two rows, 8 neighbouring values at each, the same values bit for bit.  Vectors by batches of loads (one at a time, the rows
+// without an adapter held up a call of 4099 rows, rank 16, 4096 x 4096: 31.6 us, so 25.5).
 template <typename T>
-__device__ __forceinline__ void copy8(T *out, const T *row, int n, int N, bool vec) {
+__device__ __forceinline__ void copy_rows(T *o0, T *o1, const T *y0, const T *y1, bool live0, bool live1, int n, int end, int step, int N, bool vec) {
   if (vec) {
+    constexpr int PARTS = sizeof(T) / 2, B = 8 / PARTS;
+    for (; n < end; n += B * step) {
+      uint4 v[2][B][PARTS];
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-      if (n < N) reinterpret_cast<uint4 *>(out + n)[i] = reinterpret_cast<const uint4 *>(row + n)[i];
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+#pragma unroll
+          for (int q = 0; q < PARTS; ++q)
+            if ((h ? live1 : live0) && n + i * step < min(end, N)) v[h][i][q] = __ldcs(reinterpret_cast<const uint4 *>((h ? y1 : y0) + n + i * step) + q);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+#pragma unroll
+          for (int q = 0; q < PARTS; ++q)
+            if ((h ? live1 : live0) && n + i * step < min(end, N)) reinterpret_cast<uint4 *>((h ? o1 : o0) + n + i * step)[q] = v[h][i][q];
+    }
   } else {
+    for (; n < end; n += step)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) if (n + i < N) out[n + i] = row[n + i];
+      for (int i = 0; i < 8; ++i)
+        if (n + i < N) {
+          if (live0) o0[n + i] = y0[n + i];
+          if (live1) o1[n + i] = y1[n + i];
+        }
   }
 }
 template <typename T>
@@ -261,10 +282,7 @@ lora_kernel(const lora::Args p) {
   T *o0 = static_cast<T *>(p.out) + (int64_t)r0 * p.out_stride, *o1 = o0 + 8 * p.out_stride;
   if (adapter < 0) {
     if (p.out == p.y) return;
-    for (int n = n_first + column; n < n_end; n += TM == 64 ? 32 : 128) {     // rows without an adapter
-      if (live0) copy8<T>(o0, y0, n + 8 * t, p.N, p.y_vec);
-      if (live1) copy8<T>(o1, y1, n + 8 * t, p.N, p.y_vec);
-    }
+    copy_rows<T>(o0, o1, y0, y1, live0, live1, n_first + column + 8 * t, n_end, TM == 64 ? 32 : 128, p.N, p.y_vec);     // rows without an adapter
     return;
   }
   const uint32_t base = shared_addr(smem);
@@ -543,13 +561,15 @@ struct Waves { int of[kMaxSlices + 1]; };
 
 // How a call is cut, from its sizes and the device alone: slices of K and of the columns, as many blocks of a cluster as keep the grid in one wave (75
 // tiles of rank 64 in clusters of 8, four more than there was room for, took 42 us, in clusters of 7 38 us) and 512 of K and N together in a block.
-static Plan plan_of(int64_t rows, int64_t requests, int64_t K, int64_t N, int tm, int kb, int nc, const Waves &waves) {
+// More than the 8 blocks that every GPC has room for where they are at most one an SM: one token, rank 128, 8192 x 8192 takes 11.0 us in a cluster of
+// 16 and 14.7 in one of 8, 200 tokens, rank 32, 4096 x 4096 9.5 and 12.1; with more blocks 32 tokens, rank 16, 8192 x 8192 took 11.7 and 9.6.
+static Plan plan_of(int64_t rows, int64_t requests, int64_t K, int64_t N, int tm, int kb, int nc, const Waves &waves, int sms) {
   Plan pl;
   pl.tiles = ragged_max_tiles(rows, requests, tm);
   const int64_t busy = pl.tiles - 2 < rows ? pl.tiles - 2 : rows;        // tiles of requests: at most the bound less the two of none
   pl.slices = 1;
   for (int s = 2; s <= kMaxSlices; ++s)
-    if (busy * s <= waves.of[s] && K + N >= 512 * s) pl.slices = s;
+    if (busy * s <= (s > 8 && waves.of[s] > sms ? sms : waves.of[s]) && K + N >= 512 * s) pl.slices = s;
   pl.k_slice = (int)align_up(ceil_div(K, pl.slices), kb);
   pl.n_slice = (int)align_up(ceil_div(N, pl.slices), nc);
   return pl;
@@ -575,6 +595,7 @@ static int launch_lora(Args p, int sms, cudaStream_t stream) {
   Waves waves;
   if (int e = once.get(&waves, [&](Waves &v) {
         AC4K_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        AC4K_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         cfg.numAttrs = 1;
         for (int s = 2; s <= kMaxSlices; ++s) {
           int n = 0;
@@ -586,7 +607,7 @@ static int launch_lora(Args p, int sms, cudaStream_t stream) {
         return 0;
       }))
     return e;
-  const Plan pl = plan_of(p.rows, p.requests, p.K, p.N, TM, Shrink<TM, RP>::KB, C::NC, waves);
+  const Plan pl = plan_of(p.rows, p.requests, p.K, p.N, TM, Shrink<TM, RP>::KB, C::NC, waves, sms);
   p.slices = pl.slices; p.k_slice = pl.k_slice; p.n_slice = pl.n_slice;
   cfg.gridDim = dim3((unsigned)(pl.tiles * pl.slices));
   attr[0].val.clusterDim.x = pl.slices;
