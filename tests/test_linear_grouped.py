@@ -111,6 +111,19 @@ def test_one_group_is_the_linear_layer(m, n, k):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lengths", [[100, 100, 0, 100], [129, 201, 63, 127], [125, 3, 128, 259], [385, 380, 1, 0], [53] * 40, [256, 256, 257, 511]], ids=str)
+@pytest.mark.parametrize("n,k", [(520, 576), (136, 4096)])
+def test_groups_that_fill_half_a_tile(lengths, n, k, dtype):
+    """A pair's second half has rows of the group, a few of them or none, whatever row the group begins at"""
+    from ac4k_kernel_b200 import ops
+    c = case(lengths, n, k, lead=1, behind=2, seed=n + len(lengths))
+    out = torch.full((c[0].shape[0], n), 7.0, dtype=dtype, device="cuda")
+    check(ops.linear_grouped(*c, out=out), *c)
+    assert bool((out[:1] == 7).all()) and bool((out[-2:] == 7).all())
+
+
+@gpu
 def test_a_group_is_the_same_alone_and_among_others():
     """Its rows' place, the other groups' contents (NaN scales among them) and empty groups change nothing"""
     from ac4k_kernel_b200 import ops

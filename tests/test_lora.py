@@ -62,6 +62,34 @@ def test_odd_sizes(k, n, rank, lengths):
 
 
 @gpu
+@pytest.mark.parametrize("rank", [16, 32, 64, 128])
+@pytest.mark.parametrize("lengths", [[1], [40], [200], [1] * 9, [16, 2, 30, 5], [70, 500, 3, 130], [700] * 6], ids=lambda v: f"{len(v)}x{v[0]}")
+def test_clusters_of_every_size(lengths, rank):
+    """Few tiles take a cluster of 16 blocks each, more of them smaller ones down to a single block; slices that end inside K and N"""
+    from ac4k_kernel_b200 import ops
+    c = case(lengths, [i % 3 for i in range(len(lengths))], 4872, 4424, rank, 3, seed=rank + len(lengths))
+    check(ops.lora(*c), *c)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,cut", [(2504, 0), (2504, 8), (2501, 0), (600, 4)])
+@pytest.mark.parametrize("tokens", [2, 90])
+def test_long_rows_without_an_adapter(dtype, n, cut, tokens):
+    from ac4k_kernel_b200 import ops
+    y, x, a, b, offsets, adapters, s = case([tokens] * 4, [-1, 0, -1, 1], 256, n, 16, 2, dtype, lead=3, behind=20, seed=15)
+    c = (y[:, cut:], x, a, b[:, cut:].contiguous(), offsets, adapters, s)
+    whole = torch.full((y.shape[0], n + 64), 7.0, dtype=dtype, device="cuda")
+    out = ops.lora(*c, out=whole[:, 8:8 + n - cut])
+    check(out, *c)
+    without = torch.ones(y.shape[0], dtype=torch.bool, device="cuda")
+    for i in (1, 3):
+        without[3 + i * tokens:3 + (i + 1) * tokens] = False
+    assert torch.equal(out[without], c[0][without])
+    assert bool((whole[:, :8] == 7).all()) and bool((whole[:, 8 + n - cut:] == 7).all())
+
+
+@gpu
 @pytest.mark.parametrize("tokens", [1, 6, 100])
 def test_rows_without_an_adapter_stay_as_they_are(tokens):
     """Requests without one, an index that there is no adapter of, rows in front of the first request and behind the last"""

@@ -81,7 +81,8 @@ def near_nvfp4(q, sf, g, v, layout):
 
 
 SHAPES = [(1, 8192), (1, 64), (3, 8), (5, 1), (2, 7), (17, 100), (33, 129), (130, 512), (129, 520), (9, 1024), (9, 1032), (70, 2048),
-          (11, 4096), (7, 5120), (5, 8200), (3, 16384), (3, 16392), (2, 32768), (4, 5003), (2, 32761)]
+          (11, 4096), (7, 5120), (5, 8200), (3, 16384), (3, 16392), (2, 32768), (4, 5003), (2, 32761),
+          (6, 511), (7, 514), (6, 1001), (3, 1027), (5, 2047), (5, 4095), (3, 8191), (2, 11003)]
 
 
 @gpu
