@@ -20,7 +20,9 @@ using pair::KS;
 using pair::STAGES;
 using Tile = pair::Tile<256>;
 static constexpr int kRanges = 128;                       // ranges of groups in the table
-static constexpr int SMEM_BYTES = Tile::SMEM_BYTES + (kRanges + 4) * 4;
+static constexpr int kListed = 48;                        // tiles of a pair whose places are worked out at the start
+static constexpr int LIST_BYTES = kListed * 24;
+static constexpr int SMEM_BYTES = Tile::SMEM_BYTES - 8 * pair::OUT_STAGE_BYTES /* no tile goes out through shared memory */ + (kRanges + 4) * 4 + LIST_BYTES;
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory overflow");
 
 struct Args {
@@ -35,12 +37,14 @@ struct Args {
   int tiles_n, per;              // per: groups of a range
   int row_classes;               // classes row % 4 of A in the first of its two maps (4: one map)
   bool fill;
+  bool wide;                     // rows of D begin on 32 bytes
   unsigned long long wait_ns;
 };
 
 struct TileOf {
   int group, row0, row1;         // the group's rows
   int m0, n0;                    // the tile's first row and column
+  float alpha;
 };
 
 __device__ __forceinline__ int bound_of(const Args &p, int g) { return min(max(__ldg(p.offsets + g), 0), p.rows); }
@@ -62,7 +66,11 @@ __device__ __forceinline__ TileOf tile_of(const Args &p, const volatile int *sum
   }
   int tm, tn;
   tile_coords(t - before * p.tiles_n, n, p.tiles_n, tm, tn);
-  return TileOf{g, lo, hi, (lo & ~3) + tm * pair::BMP, tn * Tile::BN};
+  return TileOf{g, lo, hi, (lo & ~3) + tm * pair::BMP, tn * Tile::BN, __fmul_rn(__ldg(p.a_gs), __ldg(p.b_gs + g * p.b_gs_stride))};
+}
+// the pair's tile number i, t in the list of all
+__device__ __forceinline__ TileOf listed_tile(const Args &p, const volatile int *sums, const TileOf *list, int i, int t) {
+  return i < kListed ? list[i] : tile_of(p, sums, t);
 }
 }  // namespace grouped_pair
 
@@ -86,8 +94,7 @@ linear_nvfp4_grouped_2cta_kernel(const __grid_constant__ CUtensorMap tma_a, cons
   const uint32_t sB = sA + STAGES * A_BYTES;
   const uint32_t sSFA = sB + STAGES * B_BYTES;
   const uint32_t sSFB = sSFA + STAGES * SFA_BYTES;
-  const uint32_t sOut = sSFB + STAGES * SFB_BYTES;     // [8 epilogue warps][32 rows x 128 B]
-  const uint32_t sBias = sOut + 8 * OUT_STAGE_BYTES;   // [8 epilogue warps][128] fp32
+  const uint32_t sBias = sSFB + STAGES * SFB_BYTES;    // [8 epilogue warps][128] fp32
   const uint32_t bars = sBias + BIAS_BYTES;
   const uint32_t full_bar = bars;                     // [STAGES] leader: operands and scales of both CTAs are in shared memory
   const uint32_t empty_bar = full_bar + 8 * STAGES;   // [STAGES] both: the MMAs that used the stage are done
@@ -96,6 +103,7 @@ linear_nvfp4_grouped_2cta_kernel(const __grid_constant__ CUtensorMap tma_a, cons
   const uint32_t shared_free_bar = tempty_bar + 16;   // leader: the 8 warps that own the shared columns have read them
   const uint32_t tmem_slot = shared_free_bar + 8;
   volatile int *sums = reinterpret_cast<volatile int *>(smem_raw + (bars + BAR_BYTES - smem_base));     // [kRanges + 1], then 3 words of scratch
+  TileOf *list = reinterpret_cast<TileOf *>(smem_raw + (bars + BAR_BYTES + (kRanges + 4) * 4 - smem_base));
   uint8_t *smem_gen = smem_raw;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -152,6 +160,10 @@ linear_nvfp4_grouped_2cta_kernel(const __grid_constant__ CUtensorMap tma_a, cons
       sums[threadIdx.x + 1] = upto;
       if (threadIdx.x == 0) sums[0] = 0;
     }
+    __syncthreads();
+    // the first tiles' places, all at once (a search of some 1000 cycles, which every role would make in front of every tile)
+    const int t = cluster_id + (int)threadIdx.x * num_clusters;
+    if (threadIdx.x < kListed && t < sums[kRanges] * p.tiles_n) list[threadIdx.x] = tile_of(p, sums, t);
   }
   tc_fence_before();
   __syncthreads();
@@ -165,8 +177,9 @@ linear_nvfp4_grouped_2cta_kernel(const __grid_constant__ CUtensorMap tma_a, cons
     const uint32_t el = elect_one();
     uint32_t s = 0, ph = 0;
     const uint32_t leader_full0 = map_to_cta(full_bar, 0);
+    int ti = 0;
     for (int t = cluster_id; t < num_tiles; t += num_clusters) {
-      const TileOf tile = tile_of(p, sums, t);
+      const TileOf tile = listed_tile(p, sums, list, ti++, t);
       const int m0 = tile.m0 + (int)rank * 128;                             // this CTA's rows of A
       const int nb0 = tile.group * p.N + tile.n0 + (int)rank * T2::B_ROWS;  // this CTA's rows of B
       const int sfb_k0 = tile.group * p.KT;
@@ -272,15 +285,13 @@ linear_nvfp4_grouped_2cta_kernel(const __grid_constant__ CUtensorMap tma_a, cons
     const int half = warp >= 10 ? 1 : 0;
     uint32_t acc_phs = 0;
     int ti = 0;
-    const float a_gs = __ldg(p.a_gs);
     const bool has_bias = p.bias != nullptr;
     const uint32_t leader_tempty = map_to_cta(tempty_bar, 0);
     const uint32_t leader_shared_free = map_to_cta(shared_free_bar, 0);
     const uint32_t bias_s = sBias + (uint32_t)(half * 4 + q) * 512u;
-    const uint32_t stage_buf = sOut + (uint32_t)(half * 4 + q) * OUT_STAGE_BYTES;
     for (int t = cluster_id; t < num_tiles; t += num_clusters) {
-      const TileOf tile = tile_of(p, sums, t);
-      const float alpha = __fmul_rn(a_gs, __ldg(p.b_gs + tile.group * p.b_gs_stride));
+      const TileOf tile = listed_tile(p, sums, list, ti, t);
+      const float alpha = tile.alpha;
       const int col0 = tile.n0 + half * 128;
       const uint32_t acc = ti & 1;
       const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + acc * ACC1_COL + half * 128;
@@ -317,27 +328,21 @@ linear_nvfp4_grouped_2cta_kernel(const __grid_constant__ CUtensorMap tma_a, cons
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(leader_tempty + 8 * acc);
-      // This warp's lane l holds row y0 + 4 l + q.  Each half (64 columns = 128 bytes of a row) goes through the staging buffer, so that a store of the
-      // warp writes 128 bytes of each of four rows.
-      const int y0 = tile.m0 + (int)rank * 128 + q;
-      T *out = static_cast<T *>(p.D);
+      // This warp's lane l holds row m0 + 4 l + q, 256 bytes of it: stored as they are, a whole sector of a row at a time.  (Through shared memory, for whole
+      // lines, the tile's stores took 3000 cycles beside the operands that come and go there.)
+      const int row = tile.m0 + (int)rank * 128 + q + 4 * lane;
+      if (row >= tile.row0 && row < tile.row1) {
+        T *out = static_cast<T *>(p.D) + (int64_t)row * p.N + col0;
 #pragma unroll
-      for (int h2 = 0; h2 < 2; ++h2) {
-        if (col0 + 64 * h2 >= p.N) break;                  // warp-uniform
-        __syncwarp();
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-          st_shared_v4u(stage_buf + lane * 128 + ((c ^ (lane & 7)) << 4), w[32 * h2 + 4 * c], w[32 * h2 + 4 * c + 1],
-                        w[32 * h2 + 4 * c + 2], w[32 * h2 + 4 * c + 3]);
-        __syncwarp();
-        const int c = lane & 7, col = col0 + 64 * h2 + c * 8;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = 4 * i + (lane >> 3), row = y0 + 4 * r;
-          uint4 v;
-          asm volatile("ld.shared::cta.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                       : "r"(stage_buf + r * 128 + ((c ^ (r & 7)) << 4)) : "memory");
-          if (row >= tile.row0 && row < tile.row1 && col < p.N) *reinterpret_cast<uint4 *>(out + (int64_t)row * p.N + col) = v;
+        for (int c = 0; c < 8; ++c) {
+          const uint32_t *v = w + 8 * c;
+          if (p.wide && col0 + 16 * c + 16 <= p.N) {
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + 16 * c), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                         "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+          } else {
+            if (col0 + 16 * c < p.N) *reinterpret_cast<uint4 *>(out + 16 * c) = make_uint4(v[0], v[1], v[2], v[3]);
+            if (col0 + 16 * c + 8 < p.N) *reinterpret_cast<uint4 *>(out + 16 * c + 8) = make_uint4(v[4], v[5], v[6], v[7]);
+          }
         }
       }
       ++ti;
@@ -410,6 +415,7 @@ int launch_linear_grouped_pair(void *D, int d_dtype, const void *A, const void *
   a.per = (int)ceil_div(groups, grouped_pair::kRanges);
   a.row_classes = M % 4 ? (int)(M % 4) : 4;
   a.fill = fill;
+  a.wide = N % 16 == 0 && (reinterpret_cast<uintptr_t>(D) & 31) == 0;
   a.wait_ns = wait_ns;
   if (a.row_classes == 4) ta_hi = ta;
   // row tiles of a group of n rows that begins up to three rows early: at most (n + 3) / 256 + 1
