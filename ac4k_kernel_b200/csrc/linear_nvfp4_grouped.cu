@@ -22,7 +22,9 @@ static constexpr int KS = 4;                     // K = 64 steps per stage (K = 
 static constexpr int W_BYTES = 128 * BKB;        // 128 weight rows x 128 bytes
 static constexpr int SF_BYTES = KS * 512;        // scale chunks of one 128-row block
 static constexpr int kThreads = 192;
-static constexpr int kPairRows = 48;             // groups of more rows than this on average go to the CTA pairs
+// Groups of more rows than this on average go to the CTA pairs, whose tiles follow one another without a gap: 64 groups of 32 rows, 2048 x 1024, take
+// 25.4 us there and 38.8 here, 128 of 16, 1024 x 2048, 37.4 and 37.9, 64 of 16, 1024 x 4096, 39.1 and 34.4, 2048 x 1024, 24.8 and 29.2.
+constexpr int pair_rows(int64_t K) { return K <= 1024 ? 8 : 24; }
 template <int NT>
 struct Cfg {
   static constexpr int X_BYTES = NT * BKB;
@@ -410,18 +412,30 @@ extern "C" int ac4k_linear_nvfp4_grouped(void *D, int d_dtype, const void *A, co
 
   const int64_t used = groups < M ? groups : M;        // groups that can have rows
   const int64_t mean = ceil_div(M, used);
-  if (mean > grouped::kPairRows && grouped_pair_takes(d_dtype, M, groups, N, K))
+  const int64_t tiles_n = ceil_div(N, 128);
+  const int k_tiles = (int)ceil_div(K / 64, grouped::KS);
+  // as many slices of K as keep one wave of blocks (two per SM), for tiles of nt rows
+  auto slices = [&](int nt) {
+    const int64_t all = ragged_max_tiles(M, used, nt) - 2, busy = all < M ? all : M;
+    int n = 1;
+    if (nt <= 64)
+      for (int cand = 4; cand >= 2; cand /= 2)
+        if (busy * tiles_n * cand <= 2 * di.sms && k_tiles / cand >= 4) { n = cand; break; }
+    while (n > 1 && ceil_div(k_tiles, ceil_div(k_tiles, n)) != n) n /= 2;   // every slice non-empty
+    return n;
+  };
+  // Long groups go to the CTA pairs, but where tiles of 64 rows are so few that K can be cut: 4 groups of 175 rows, 1024 x 8192, take 15.2 us cut and
+  // 19.0 in pairs, 2 of 150 11.3 and 18.4, 8 of 125, 512 x 4096, 11.2 and 13.1, 4 of 175, 1024 x 2048, 10.3 both; uncut, 4 of 250, 2048 x 4096,
+  // 14.9 and 14.4.
+  const int cut = mean > grouped::pair_rows(K) ? slices(64) : 1;
+  if (mean > grouped::pair_rows(K) && cut == 1 && grouped_pair_takes(d_dtype, M, groups, N, K))
     return launch_linear_grouped_pair(D, d_dtype, A, A_sf, A_gs, B, B_sf, B_gs, b_gs_per_group ? 1 : 0, bias, bias_dtype, offsets, fill != 0, M, groups, N,
                                       K, di.sms, status, debug_wait_ns() ? debug_wait_ns() : kWaitTimeoutNs, stream);
-  const int nt = mean <= 16 ? 16 : (mean <= 32 ? 32 : (mean <= 64 ? 64 : 128));
-  const int64_t tiles_n = ceil_div(N, 128);
-  const int64_t tiles = ragged_max_tiles(M, used, nt), busy = tiles - 2 < M ? tiles - 2 : M;
-  const int k_tiles = (int)ceil_div(K / 64, grouped::KS);
-  int splits = 1;
-  if (nt <= 64)
-    for (int cand = 4; cand >= 2; cand /= 2)      // as many slices as keep one wave of blocks (two per SM)
-      if (busy * tiles_n * cand <= 2 * di.sms && k_tiles / cand >= 4) { splits = cand; break; }
-  while (splits > 1 && ceil_div(k_tiles, ceil_div(k_tiles, splits)) != splits) splits /= 2;   // every slice non-empty
+  // Tiles of twice the mean: a group a little above it would have two, and stream its weights twice (64 groups of 16 rows, 1024 x 4096: 36.1 us in
+  // tiles of 16, 34.4 in tiles of 32; 8 groups of 12, 8192 x 4096: 35.6 and 32.0)
+  const int nt = mean <= 8 ? 16 : (mean <= 16 ? 32 : (mean <= 64 || cut > 1 ? 64 : 128));
+  const int64_t tiles = ragged_max_tiles(M, used, nt);
+  const int splits = slices(nt);
   if (tiles * tiles_n * splits > 0x7FFFFFFFLL) return fail(AC4K_ERR_SHAPE, "too many tiles");
   CUtensorMap tx, tw;
   if (int e = make_tmap(A, M, K / 2, nt, &tx)) return e;
