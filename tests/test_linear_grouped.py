@@ -1,7 +1,7 @@
 """`linear_grouped`: NVFP4 products with a weight per group of rows, against the products of the values that the codes stand for in 64 bits.
 
 Bounds.  A product of two codes and their scales is exact in fp32; the sum over K takes one MMA of 64 products after another into an fp32
-accumulator, each within 2^-22 of the terms so far, so 2^-16 of the sum of magnitudes for the K <= 4096 of these tests; alpha and bias round twice
+accumulator, each within 2^-22 of the terms so far, so 2^-16 of the sum of magnitudes for the K <= 4096 of these tests (2^-14 for the one of 16384, held to the same); alpha and bias round twice
 more (2^-23); then one rounding to out: half a step, 2^-8 of the value for bf16, 2^-11 (2^-25 among its subnormals) for fp16, 2^-24 for fp32."""
 import sys
 
@@ -138,6 +138,24 @@ def test_a_group_is_the_same_alone_and_among_others():
     other = ops.linear_grouped(x, sf, x_g, w, wsf, w_g, offsets)
     assert torch.equal(other[7:97], out[7:97])
     assert bool(other[:7].isnan().all()) and bool(other[97:].isnan().all())
+
+
+@gpu
+@pytest.mark.parametrize("each", [1, 40])
+def test_weights_past_32_bits(each):
+    """5.4 GB of codes: the last groups' weights begin behind 2^32 bytes"""
+    from ac4k_kernel_b200 import ops
+    e, n, k = 40, 16384, 16384
+    x = ops.quantize(gaussian((e * each, k), 41).cuda(), 0, 1)
+    w = torch.randint(0, 256, (e, n, k // 2), dtype=torch.uint8, device="cuda")
+    w_sf = torch.randint(0x28, 0x40, (e, k // 64, n, 4), dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    w_g = torch.tensor(0.01, device="cuda")
+    offsets = torch.arange(0, e * each + 1, each, dtype=torch.int32, device="cuda")
+    out = ops.linear_grouped(*x, w, w_sf, w_g, offsets)
+    for g in (0, e - 2, e - 1):
+        for n0 in (0, n - 256):
+            part = torch.tensor([each * g, each * (g + 1)], dtype=torch.int32)
+            check(out[:, n0:n0 + 256], *x, w[g:g + 1, n0:n0 + 256], w_sf[g:g + 1, :, n0:n0 + 256], w_g, part)
 
 
 @gpu

@@ -146,6 +146,24 @@ def test_strides(dtype, cut):
 
 
 @gpu
+@pytest.mark.parametrize("requests", [1, 20000])
+def test_rows_past_32_bits(requests):
+    """The last rows of x, y and out begin behind 2^32 bytes"""
+    from ac4k_kernel_b200 import ops
+    t, k, n = 300000, 8192, 8192
+    x = torch.randn((t, k), dtype=torch.bfloat16, device="cuda")
+    y = torch.randn((t, n), dtype=torch.bfloat16, device="cuda")
+    _, _, a, b, _, _, s = case([1], [0], k, n, 16, 2, seed=16)
+    offsets = torch.linspace(0, t, requests + 1, dtype=torch.float64).long()
+    adapters = torch.arange(requests) % 2
+    out = ops.lora(y, x, a, b, offsets.int().cuda(), adapters.int().cuda(), s)
+    for lo in (0, t // 2, t - 300):
+        which = torch.searchsorted(offsets, torch.arange(lo, lo + 300), right=True) - 1
+        rows = slice(lo, lo + 300)
+        check(out[rows], y[rows], x[rows], a, b, torch.arange(301), adapters[which], s)
+
+
+@gpu
 def test_many_requests():
     """More requests than threads of a block, most of them empty"""
     from ac4k_kernel_b200 import ops

@@ -134,6 +134,21 @@ def test_many_rows(k, residual, weight):
 
 
 @gpu
+@pytest.mark.parametrize("k", [16384, 16381])
+def test_rows_past_32_bits(k):
+    """The last rows of every tensor begin behind 2^32 bytes"""
+    from ac4k_kernel_b200 import ops
+    m = 270000
+    x = torch.randn((m, k), dtype=torch.bfloat16, device="cuda")
+    _, w, _ = inputs(1, k, seed=2)
+    out, sf, total = ops.rms_norm(x, w, 1e-6, residual=x, precision="fp8e4m3")
+    for lo in (0, m - 100):
+        s, v = formula(x[lo:lo + 100], w, x[lo:lo + 100], 1e-6)
+        assert torch.equal(total[lo:lo + 100], (x[lo:lo + 100].float() * 2).bfloat16())
+        near_fp8(out[lo:lo + 100], torch.cat([sf[lo:lo + 100], torch.zeros(12, device="cuda")]), v)
+
+
+@gpu
 @pytest.mark.parametrize("k", [64, 100, 1024, 2048, 4096, 8192, 16384, 32768])
 @pytest.mark.parametrize("precision", [None, "fp8e4m3", "nvfp4"])
 def test_a_row_is_the_same_alone_and_in_a_batch(k, precision):
