@@ -146,6 +146,40 @@ def test_strides(dtype, cut):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rank", [4, 16, 32, 64, 128])
+@pytest.mark.parametrize("requests,count,longest", [(2, 1, 1), (9, 1, 1), (50, 3, 1), (129, 64, 2), (254, 5, 3), (255, 5, 3), (40, 2, 30), (64, 20, 1)])
+def test_requests_that_share_adapters(requests, count, longest, rank, dtype):
+    """Rows of one adapter from all over the batch, empty requests, requests without an adapter and rows of no request among them"""
+    from ac4k_kernel_b200 import ops
+    g = torch.Generator().manual_seed(requests + rank)
+    lengths = torch.randint(0 if longest > 1 else 1, longest + 1, (requests,), generator=g).tolist()
+    adapters = torch.randint(-1 if requests > 9 else 0, count + (requests > 50), (requests,), generator=g).tolist()
+    y, x, a, b, offsets, which, s = case(lengths, adapters, 712, 392, rank, count, dtype, lead=5, behind=19, seed=requests)
+    x[:5], x[-19:] = float("nan"), float("nan")
+    c = (y[:, 8:], x[:, 8:], a[:, :, 8:].contiguous(), b[:, 8:].contiguous(), offsets, which, s)
+    out = ops.lora(*c)
+    inside = torch.zeros(y.shape[0], dtype=torch.bool, device="cuda")
+    inside[5:-19] = True
+    check(out[inside], c[0][inside], c[1][inside], *c[2:4], offsets - 5, which, s)
+    assert torch.equal(out[~inside], c[0][~inside])
+    assert torch.equal(ops.lora(*c, out=c[0]), out) and torch.equal(ops.lora(*c[:2], *c[2:], out=torch.empty_like(out)), ops.lora(*c))
+
+
+@gpu
+def test_offsets_that_are_none_with_shared_adapters():
+    from ac4k_kernel_b200 import ops
+    y, x, a, b, _, adapters, s = case([10] * 6, [0, 1, 0, 1, -1, 0], 64, 48, 8, 2, seed=18)
+    big = torch.full((180, 48), 7.0, dtype=y.dtype, device="cuda")
+    for bad in ([-5, 10, 20, 30, 40, 50, 60], [0, 10, 20, 1000000, 5, 60, 60], [0, 20, 10, 30, 0, 60, 1], [60, 50, 40, 30, 20, 10, 0],
+                [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, 5, 2 ** 31 - 1, -7, 60]):
+        offsets = torch.tensor(bad, dtype=torch.int32, device="cuda")
+        ops.lora(y, x, a, b, offsets, adapters, s, out=big[60:120])
+        torch.cuda.synchronize()
+        assert bool((big[:60] == 7).all()) and bool((big[120:] == 7).all())
+
+
+@gpu
 @pytest.mark.parametrize("requests", [1, 20000])
 def test_rows_past_32_bits(requests):
     """The last rows of x, y and out begin behind 2^32 bytes"""
