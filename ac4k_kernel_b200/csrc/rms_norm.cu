@@ -136,9 +136,18 @@ __device__ __forceinline__ void reduce_row(float &sum, float &amax, float *part)
 
 }  // namespace norm
 
+namespace norm {
+// Blocks on an SM that the compiler is to leave registers for: as many rows in flight as a row's 8 C values and its two loads of 4 C words allow.
+// Left to itself it took 86 registers for C = 5, and 4099 rows of 5120 (bf16 residual, e4m3 out) 28.3 us, now 27.0; without a residual 20.9 and 18.1; 6144
+// 37.0 and 35.4; 12288 69.1 and 62.8.  (8 blocks for C = 5 spill: 29.2.)
+constexpr int blocks_for(int c, int threads) {
+  return c == 8 ? 512 / threads : (c == 6 ? 768 / threads : (c == 5 ? 896 / threads : (c == 4 ? 1024 / threads : 1)));
+}
+}  // namespace norm
+
 // Rows of 16-byte vectors: G threads share a row (a warp, or the block), C chunks of 8 elements in registers each.
 template <int FMT, int G, int C, int THREADS>
-__global__ void __launch_bounds__(THREADS, C == 8 ? 512 / THREADS : 1)
+__global__ void __launch_bounds__(THREADS, norm::blocks_for(C, THREADS))
 rms_norm_kernel(const norm::Args p) {
   using namespace norm;
   static_assert(G == 32 || G == THREADS, "a row per warp or per block");
