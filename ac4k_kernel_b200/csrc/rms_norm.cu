@@ -87,12 +87,17 @@ __device__ __forceinline__ void weight8(const Args &p, int at, float (&w)[8]) {
 __device__ __forceinline__ float rstd_of(float sum, const Args &p) {
   return __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum, (float)p.K), p.eps)));
 }
-// Scale of an e4m3 row and the factor its elements take.  A row of zeros has the scale 0 and codes 0, and so has one whose largest
-// value is so small (below 2^-117) that the factor would pass fp32's range.
-__device__ __forceinline__ float e4m3_scale(float amax, float &r) {
-  r = __fdiv_rn(kE4m3Max, amax);
-  if (amax < 0x1p-117f) { r = 0.0f; return 0.0f; }
-  return __fdiv_rn(amax, kE4m3Max);
+// Scale of an e4m3 row with the maximum `amax` of |s * weight|, and the factors that its elements take in front of the weight and behind it.  rstd is in
+// an element and in the row's maximum alike, so a code is s * weight times 448 over that maximum: two roundings less than by way of v, half as many
+// codes on the other side of a border.  By way of v where that maximum or rstd are beyond what fp32 holds.  A row of zeros has the scale 0 and
+// codes 0, and so has one whose largest value is so small (below 2^-117) that the factor would pass fp32's range.
+struct RowScale { float scale, pre, r; };
+__device__ __forceinline__ RowScale e4m3_scale(float amax, float rstd) {
+  const float top = __fmul_rn(amax, rstd);
+  RowScale q{__fdiv_rn(top, kE4m3Max), rstd, __fdiv_rn(kE4m3Max, top)};
+  if (top < 0x1p-117f) q.scale = q.r = 0.0f;
+  else if (amax >= 0x1p-117f && amax < INFINITY && top < INFINITY) { q.pre = 1.0f; q.r = __fdiv_rn(kE4m3Max, amax); }
+  return q;
 }
 
 // byte offset of the scale word (four blocks of 16) of row `row`, K step `k64`
@@ -138,8 +143,8 @@ __device__ __forceinline__ void reduce_row(float &sum, float &amax, float *part)
 
 namespace norm {
 // Blocks on an SM that the compiler is to leave registers for: as many rows in flight as a row's 8 C values and its two loads of 4 C words allow.
-// Left to itself it took 86 registers for C = 5, and 4099 rows of 5120 (bf16 residual, e4m3 out) 28.3 us, now 27.0; without a residual 20.9 and 18.1; 6144
-// 37.0 and 35.4; 12288 69.1 and 62.8.  (8 blocks for C = 5 spill: 29.2.)
+// Left to itself it took 86 registers for C = 5, and 4099 rows of 5120 (bf16 residual, e4m3 out) 28.3 us, now 27.4; without a residual 20.9 and 19.0; 6144
+// 37.0 and 35.2; 12288 69.1 and 62.8.  (8 blocks for C = 5 spill: 29.2.)
 constexpr int blocks_for(int c, int threads) {
   return c == 8 ? 512 / threads : (c == 6 ? 768 / threads : (c == 5 ? 896 / threads : (c == 4 ? 1024 / threads : 1)));
 }
@@ -236,20 +241,20 @@ rms_norm_kernel(const norm::Args p) {
   sum = __fadd_rn(sum, odd);
   reduce_row<G>(sum, amax, part);
   const float rstd = rstd_of(sum, p);
-  float r = 0.0f, alpha = 0.0f;
+  RowScale q = {};
+  float alpha = 0.0f;
   if (FMT == kE4m3) {
-    const float scale = e4m3_scale(__fmul_rn(amax, rstd), r);
-    if (t == 0) reinterpret_cast<float *>(p.sf)[row] = scale;
+    q = e4m3_scale(amax, rstd);
+    if (t == 0) reinterpret_cast<float *>(p.sf)[row] = q.scale;
   }
   if (FMT == kNvfp4) alpha = load_alpha(p.gs);
   const int64_t Kp = FMT == kBf16 ? p.K : (FMT == kE4m3 ? align_up(p.K, 16) : align_up(p.K, 64));
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int ch = c * G + t;
-    float v[8] = {};
-    if (ch < nfull) {
-      float w[8];
-      weight8(p, ch * 8, w);
+    float v[8] = {}, w[8] = {};
+    if (ch < nfull) weight8(p, ch * 8, w);
+    if (ch < nfull && (FMT != kE4m3 || p.normed != nullptr)) {
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
         v[i] = s[c][i]; v[i + 1] = s[c][i + 1];
@@ -264,7 +269,15 @@ rms_norm_kernel(const norm::Args p) {
     if (p.normed != nullptr && ch < nfull) *reinterpret_cast<uint4 *>(p.normed + row * p.K + ch * 8) = pack8(v);
     if (FMT == kE4m3) {
 #pragma unroll
-      for (int i = 0; i < 8; i += 2) mul2(v[i], v[i + 1], r, r);
+      for (int i = 0; i < 8; ++i) v[i] = s[c][i];
+      if (q.pre != 1.0f)              // (seldom, and the whole row alike)
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) mul2(v[i], v[i + 1], q.pre, q.pre);
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        mul2(v[i], v[i + 1], w[i], w[i + 1]);
+        mul2(v[i], v[i + 1], q.r, q.r);
+      }
       if (ch * 8 < Kp)
         *reinterpret_cast<uint2 *>(p.out + row * Kp + ch * 8) = make_uint2(f32x4_to_e4m3x4(v[0], v[1], v[2], v[3]), f32x4_to_e4m3x4(v[4], v[5], v[6], v[7]));
     }
@@ -352,10 +365,11 @@ rms_norm_any_kernel(const norm::Args p) {
     for (int i = t; i < K; i += T) wide[i] = __float2bfloat16_rn(__fmul_rn(__fmul_rn(row_s[i], rstd), weight(i)));
   }
   if (FMT == kBf16) return;
-  float r = 0.0f, alpha = 0.0f;
+  RowScale q = {};
+  float alpha = 0.0f;
   if (FMT == kE4m3) {
-    const float scale = e4m3_scale(__fmul_rn(amax, rstd), r);
-    if (t == 0) reinterpret_cast<float *>(p.sf)[row] = scale;
+    q = e4m3_scale(amax, rstd);
+    if (t == 0) reinterpret_cast<float *>(p.sf)[row] = q.scale;
   }
   if (FMT == kNvfp4) alpha = load_alpha(p.gs);
   const int Kp = (int)(FMT == kE4m3 ? align_up(K, 16) : align_up(K, 64));
@@ -366,10 +380,10 @@ rms_norm_any_kernel(const norm::Args p) {
       const float4 s = *reinterpret_cast<const float4 *>(row_s + i);
       const float f[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = i + j < K ? __fmul_rn(__fmul_rn(f[j], rstd), weight(i + j)) : 0.0f;
+      for (int j = 0; j < 4; ++j) v[j] = i + j < K ? __fmul_rn(__fmul_rn(f[j], FMT == kE4m3 ? q.pre : rstd), weight(i + j)) : 0.0f;
     }
     if (FMT == kE4m3) {
-      if (i < Kp) *reinterpret_cast<uint32_t *>(p.out + row * Kp + i) = f32x4_to_e4m3x4(__fmul_rn(v[0], r), __fmul_rn(v[1], r), __fmul_rn(v[2], r), __fmul_rn(v[3], r));
+      if (i < Kp) *reinterpret_cast<uint32_t *>(p.out + row * Kp + i) = f32x4_to_e4m3x4(__fmul_rn(v[0], q.r), __fmul_rn(v[1], q.r), __fmul_rn(v[2], q.r), __fmul_rn(v[3], q.r));
     }
     if (FMT == kNvfp4) {
       float m = max_nan(max_nan(fabsf(v[0]), fabsf(v[1])), max_nan(fabsf(v[2]), fabsf(v[3])));

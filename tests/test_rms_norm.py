@@ -318,7 +318,8 @@ def test_refusals_of_the_c_interface():
     for kw, code in ((dict(precision=3), -4), (dict(layout=2), -4), (dict(rdt=1), -4), (dict(wdt=1), -4), (dict(m=-1), -2), (dict(k=0), -2),
                      (dict(xs=-64), -2), (dict(k=32769), -5), (dict(eps=-1.0), -2), (dict(eps=math.nan), -2), (dict(out=None), -1), (dict(x=None), -1),
                      (dict(sf=None), -1), (dict(gs=None), -1), (dict(residual=None), -1), (dict(precision=0, normed=P), -5), (dict(x=P + 1), -3),
-                     (dict(residual=P + 2, rdt=2), -3), (dict(weight=P + 1), -3), (dict(sf=P + 2), -3), (dict(m=1 << 40), -2)):
+                     (dict(residual=P + 2, rdt=2), -3), (dict(weight=P + 1), -3), (dict(sf=P + 2), -3), (dict(m=1 << 40), -2),
+                     (dict(out=P + 2), -3), (dict(out=P + 2, precision=1), -3), (dict(out=P + 1, precision=0), -3)):
         assert call(**kw) == code, kw
         assert last_error()
     assert call(m=0, out=None) == 0
