@@ -18,6 +18,8 @@
 // of a thread over four MMAs are neighbours, which it loads from y and stores in vectors.
 //
 // A x is summed in fp32 and handed over as two bf16 values (16 bits of mantissa together), for which the second half takes two MMAs.
+// Both have the sign of A x, and neither is zero unless it is (or is below 2^-110): an infinite B gives infinity from each, and not 0 * infinity or
+// infinity - infinity, which the formula does not have.
 #include "ragged.cuh"
 #include "sm100_ptx.cuh"
 
@@ -95,6 +97,20 @@ __device__ __forceinline__ int adapter_of(const Args &p, const RaggedTile &t) {
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// The bf16 next below a finite a's magnitude, with its sign (strictly below, but for zeros): what is left is at most a unit in its last place, and has
+// a's sign.  a itself where it is not finite.
+__device__ __forceinline__ float below_bf16(float a) {
+  const uint32_t u = __float_as_uint(a), m = u & 0x7FFFFFFFu;
+  if (m >= 0x7F800000u) return a;
+  return __uint_as_float((u & 0x80000000u) | (m ? (m - 1) & 0xFFFF0000u : 0u));
+}
+// a in two bf16 parts, the larger one in the low half: within 2^-16 of it (the rest, at most 2^-7 of a's power of two, is rounded to eight bits, by half
+// a step of 2^-8 at most)
+__device__ __forceinline__ uint32_t two_parts(float a) {
+  const float h = below_bf16(a);
+  return pack_bf16(h, isfinite(a) ? __fsub_rn(a, h) : a);         // (the difference is exact)
 }
 }  // namespace lora
 
@@ -454,9 +470,7 @@ lora_kernel(const lora::Args p) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         // (behind the rank: not 0 * infinity, which is what an infinity in x has left there)
-        const float a = i % RP + e < p.R ? __fmul_rn(f[e], scale) : 0.0f;
-        const float h = __bfloat162float(__float2bfloat16_rn(a));
-        u[e] = pack_bf16(h, isfinite(h) ? __fsub_rn(a, h) : 0.0f);        // (the difference is exact)
+        u[e] = two_parts(i % RP + e < p.R ? __fmul_rn(f[e], scale) : 0.0f);
       }
       for (int q = 0; q < p.slices; ++q) {
         const uint32_t at = p.slices > 1 ? ptx::map_to_cta(total + i * 4, q) : total + i * 4;

@@ -128,6 +128,34 @@ def test_nan_stays_in_its_row_and_its_adapter():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rank", [3, 16, 40, 128])
+@pytest.mark.parametrize("exact", [True, False])
+def test_infinite_weights_give_infinities(exact, rank, dtype):
+    """An infinite B takes its sign from A x, whatever A x leaves behind where it is cut into parts of 8 bits: nothing (`exact`: A x are 7-bit
+    numbers, some of them 0) or a rest of the one or the other sign.  NaN only where the formula has 0 * infinity or infinities of both signs."""
+    from ac4k_kernel_b200 import ops
+    y, x, a, b, offsets, adapters, _ = case([1, 7, 90], [0, 1, 0], 256, 136, rank, 2, dtype, seed=rank)
+    if exact:
+        x = (torch.arange(x.numel(), device="cuda").reshape(x.shape) * 37 % 129 - 64).bfloat16()
+        a.zero_()
+        for r in range(rank):
+            a[:, r, (5 * r + 1) % 256] = 1.0
+    for j in range(2):
+        b[j, 3, 0] = float("inf")
+        b[j, 4, 1] = -float("inf")
+        b[j, 70, 0], b[j, 70, 2] = float("inf"), float("inf")
+        b[j, 135, rank - 1] = float("inf")
+    want, lo = y.double().clone(), offsets.tolist()
+    for i, j in enumerate(adapters.tolist()):
+        low = x[lo[i]:lo[i + 1]].double() @ a[j].double().t()
+        want[lo[i]:lo[i + 1]] += (low[:, None, :] * b[j].double()).sum(-1)        # (no product that a library skips)
+    out = ops.lora(y, x, a, b, offsets, adapters).double()
+    assert torch.equal(out.isnan(), want.isnan())
+    assert torch.equal(out == float("inf"), want == float("inf")) and torch.equal(out == -float("inf"), want == -float("inf"))
+    assert bool(want.isinf().any()) and (not exact or bool(want.isnan().any()))
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("cut", [0, 1, 8])
 def test_strides(dtype, cut):
