@@ -17,9 +17,10 @@
 // operands, and needs no ldmatrix; the columns of the second half are dealt so that the 8 results
 // of a thread over four MMAs are neighbours, which it loads from y and stores in vectors.
 //
-// A x is summed in fp32 and handed over as two bf16 values (16 bits of mantissa together), for which the second half takes two MMAs.
-// Both have the sign of A x, and neither is zero unless it is (or is below 2^-110): an infinite B gives infinity from each, and not 0 * infinity or
-// infinity - infinity, which the formula does not have.
+// A x is summed in fp32 and handed over as two bf16 values (16 bits of mantissa together: below the rounding of a 16-bit y), for which the second half
+// takes two MMAs; for an fp32 y as three, all of its bits (2000 rows, rank 128, 4096 x 4096: 58 us, with two 51; 8192 rows, rank 32, 8192 x 8192: 179
+// both).  They have the sign of A x, and none is zero unless it is (or is below 2^-110): an infinite B gives infinity from each, and not
+// 0 * infinity or infinity - infinity, which the formula does not have.
 #include "ragged.cuh"
 #include "sm100_ptx.cuh"
 
@@ -99,18 +100,29 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// The bf16 next below a finite a's magnitude, with its sign (strictly below, but for zeros): what is left is at most a unit in its last place, and has
-// a's sign.  a itself where it is not finite.
-__device__ __forceinline__ float below_bf16(float a) {
-  const uint32_t u = __float_as_uint(a), m = u & 0x7FFFFFFFu;
-  if (m >= 0x7F800000u) return a;
-  return __uint_as_float((u & 0x80000000u) | (m ? (m - 1) & 0xFFFF0000u : 0u));
+// Takes a bf16 part off a finite a: its first eight bits, or half of a where it has no more, so that the part and what is left both have a's sign and
+// are exact.  Of one that is not finite both are a itself.
+__device__ __forceinline__ float take_part(float &a) {
+  if (!isfinite(a)) return a;
+  float h = __uint_as_float(__float_as_uint(a) & 0xFFFF0000u);
+  if (h == a) h = __fmul_rn(a, 0.5f);
+  a = __fsub_rn(a, h);
+  return h;
 }
 // a in two bf16 parts, the larger one in the low half: within 2^-16 of it (the rest, at most 2^-7 of a's power of two, is rounded to eight bits, by half
 // a step of 2^-8 at most)
 __device__ __forceinline__ uint32_t two_parts(float a) {
-  const float h = below_bf16(a);
-  return pack_bf16(h, isfinite(a) ? __fsub_rn(a, h) : a);         // (the difference is exact)
+  const float h = take_part(a);
+  return pack_bf16(h, a);
+}
+// two values in three bf16 parts each, the whole of them: 24 bits by eight at a time
+__device__ __forceinline__ void three_parts(float a, float b, uint32_t (&parts)[3]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float ha = take_part(a), hb = take_part(b);
+    parts[i] = pack_bf16(ha, hb);
+  }
+  parts[2] = pack_bf16(a, b);
 }
 }  // namespace lora
 
@@ -446,7 +458,7 @@ lora_kernel(const lora::Args p) {
   }
   // ------------------------------------------------------------------ the sums of all slices
   // The blocks of the cluster take a share of the values each, add them in the order of the slices, scale and round them to two bf16 parts (a value
-  // in the low half of a word, what it leaves in the high one) and write them to every block.
+  // in the low half of a word, what it leaves in the high one) and write them to every block; as they are where there will be three parts.
   const uint32_t total = base + S2::SUMS;
   {
     constexpr int WARPS = TM == 64 ? 1 : 4;               // sums of a row
@@ -470,7 +482,8 @@ lora_kernel(const lora::Args p) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         // (behind the rank: not 0 * infinity, which is what an infinity in x has left there)
-        u[e] = two_parts(i % RP + e < p.R ? __fmul_rn(f[e], scale) : 0.0f);
+        const float a = i % RP + e < p.R ? __fmul_rn(f[e], scale) : 0.0f;
+        u[e] = sizeof(T) == 4 ? __float_as_uint(a) : two_parts(a);
       }
       for (int q = 0; q < p.slices; ++q) {
         const uint32_t at = p.slices > 1 ? ptx::map_to_cta(total + i * 4, q) : total + i * 4;
@@ -482,9 +495,10 @@ lora_kernel(const lora::Args p) {
   }
   // ------------------------------------------------------------------ y + B of the sum over the block's columns
   constexpr int KC = RP / 32 > 0 ? RP / 32 : 1;      // steps of 32 k (one of 16 for rank 16)
-  // Both parts of A x for this warp's rows: the fragments of a step of 32 k hold k = 8 t + {0, 1}, {2, 3} (first MMA) and {4, 5}, {6, 7} (second);
+  // The parts of A x for this warp's rows: the fragments of a step of 32 k hold k = 8 t + {0, 1}, {2, 3} (first MMA) and {4, 5}, {6, 7} (second);
   // rank 16: k = 4 t + {0, 1}, {2, 3}.  Pair i -> MMA i / 2, k half i % 2; registers {row g, row g + 8} x {k half}
-  uint32_t hi[KC][2][4], lo[KC][2][4];
+  constexpr int CUTS = sizeof(T) == 4 ? 3 : 2;
+  uint32_t part[CUTS][KC][2][4];
   constexpr int PER = RP == 16 ? 4 : 8;
 #pragma unroll
   for (int c = 0; c < KC; ++c)
@@ -495,8 +509,16 @@ lora_kernel(const lora::Args p) {
       for (int q = 0; q < PER / 4; ++q) {
         v[q] = make_uint4(0, 0, 0, 0);
         if (h ? live1 : live0) v[q] = lds16(total + (uint32_t)((r0 - tile.row0 + 8 * h) * RP + c * 32 + PER * t + 4 * q) * 4u);
-        hi[c][q][h] = __byte_perm(v[q].x, v[q].y, 0x5410); lo[c][q][h] = __byte_perm(v[q].x, v[q].y, 0x7632);
-        hi[c][q][2 + h] = __byte_perm(v[q].z, v[q].w, 0x5410); lo[c][q][2 + h] = __byte_perm(v[q].z, v[q].w, 0x7632);
+        if constexpr (CUTS == 3) {
+          uint32_t a[3], b[3];
+          three_parts(__uint_as_float(v[q].x), __uint_as_float(v[q].y), a);
+          three_parts(__uint_as_float(v[q].z), __uint_as_float(v[q].w), b);
+#pragma unroll
+          for (int i = 0; i < 3; ++i) { part[i][c][q][h] = a[i]; part[i][c][q][2 + h] = b[i]; }
+        } else {
+          part[0][c][q][h] = __byte_perm(v[q].x, v[q].y, 0x5410); part[1][c][q][h] = __byte_perm(v[q].x, v[q].y, 0x7632);
+          part[0][c][q][2 + h] = __byte_perm(v[q].z, v[q].w, 0x5410); part[1][c][q][2 + h] = __byte_perm(v[q].z, v[q].w, 0x7632);
+        }
       }
     }
   __syncthreads();              // all have read the sums: their place is the ring's now
@@ -530,16 +552,16 @@ lora_kernel(const lora::Args p) {
         // columns of MMA j: g -> n + 8 (g / 2) + 2 j + g % 2, so that this thread's results (columns 2 t, 2 t + 1 of each) are n + 8 t + 2 j, + 1
         if (RP == 16) {
           const uint2 w = lds8(b_from[j] + now + u * 32 * S2::CH * 16);
-          mma_bf16(acc[j], hi[0][0][0], hi[0][0][1], hi[0][0][2], hi[0][0][3], w.x, w.y);
-          mma_bf16(acc[j], lo[0][0][0], lo[0][0][1], lo[0][0][2], lo[0][0][3], w.x, w.y);
+#pragma unroll
+          for (int i = 0; i < CUTS; ++i) mma_bf16(acc[j], part[i][0][0][0], part[i][0][0][1], part[i][0][0][2], part[i][0][0][3], w.x, w.y);
         } else {
 #pragma unroll
           for (int c = 0; c < KC; ++c) {
             const uint4 w = lds16((b_from[j] ^ (S2::CH >= 8 ? (c & 1) * 64 : 0)) + (c >> 1) * 128 + now + u * 32 * S2::CH * 16);
-            mma_bf16(acc[j], hi[c][0][0], hi[c][0][1], hi[c][0][2], hi[c][0][3], w.x, w.y);
-            mma_bf16(acc[j], lo[c][0][0], lo[c][0][1], lo[c][0][2], lo[c][0][3], w.x, w.y);
-            mma_bf16(acc[j], hi[c][1][0], hi[c][1][1], hi[c][1][2], hi[c][1][3], w.z, w.w);
-            mma_bf16(acc[j], lo[c][1][0], lo[c][1][1], lo[c][1][2], lo[c][1][3], w.z, w.w);
+#pragma unroll
+            for (int i = 0; i < CUTS; ++i) mma_bf16(acc[j], part[i][c][0][0], part[i][c][0][1], part[i][c][0][2], part[i][c][0][3], w.x, w.y);
+#pragma unroll
+            for (int i = 0; i < CUTS; ++i) mma_bf16(acc[j], part[i][c][1][0], part[i][c][1][1], part[i][c][1][2], part[i][c][1][3], w.z, w.w);
           }
         }
       }

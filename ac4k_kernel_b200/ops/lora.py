@@ -17,7 +17,10 @@ def lora(y, x, a, b, offsets, adapters, scaling=None, *, out=None):
     [adapters, N, R], bf16, contiguous, R at most 128 (an adapter of a lower rank has zeros behind it).  offsets: int32 [requests + 1],
     ascending: the rows of request i are offsets[i] to offsets[i + 1]; adapters: int32 [requests], the adapter of each, negative for none;
     scaling: fp32 [adapters], None for ones.  Rows without an adapter and rows of no request are those of y.
-    out: None, y itself, or a tensor like y that overlaps neither y nor x.  Returns out."""
+    out: None, y itself, or a tensor like y that overlaps neither y nor x.  Returns out.
+
+    x A^T is summed in fp32 and its product with B in fp32, with 16 bits of each value of x A^T for a bf16 or fp16 y and all of them for an fp32 y; out
+    is rounded once.  A y that `linear()` made in bf16 was rounded there before: where one rounding in all is wanted, give `linear()` an fp32 out."""
     if host_calls is not None:
         made = host_calls.lora(y, x, a, b, offsets, adapters, scaling, out)
         if made is not None:

@@ -278,7 +278,8 @@ int ac4k_rms_norm(void *out, void *sf, const float *global_scale, int precision,
  *   stride) or overlaps it nowhere.  a: bf16 [n_adapters, R, K], b: bf16 [n_adapters, N, R], dense; an adapter of a lower rank has zeros
  *   behind it.  offsets: int32 [requests + 1], ascending within [0, rows]; adapters: int32 [requests]; scaling: fp32 [n_adapters] or NULL
  *   (ones); all on the device.  R <= 128.
- * out does not overlap x either.  A x is held in fp32 and its product with B in fp32 with 16 bits of each value of A x; one rounding to out. */
+ * out does not overlap x either.  A x is held in fp32 and its product with B in fp32, with 16 bits of each value of A x for a bf16 or fp16 y and all of
+ * them for an fp32 y; one rounding to out. */
 int ac4k_lora(void *out, const void *y, int y_dtype, const void *x, const void *a, const void *b, const int32_t *offsets,
               const int32_t *adapters, const float *scaling, int64_t rows, int64_t requests, int64_t n_adapters, int64_t K, int64_t N,
               int64_t R, int64_t x_stride, int64_t y_stride, int64_t out_stride, ac4k_stream_t stream);

@@ -50,6 +50,28 @@ def test_against_the_formula(dtype, rank, lengths):
     c = case(lengths, [i % 3 for i in range(len(lengths))], 640, 328, rank, 3, dtype, seed=rank)
     check(ops.lora(*c), *c)
 
+@gpu
+@pytest.mark.parametrize("rank", [1, 16, 24, 64, 128])
+@pytest.mark.parametrize("lengths", [[1], [1, 1, 5, 2], [100], [64, 130]], ids=str)
+@pytest.mark.parametrize("k,n", [(512, 328), (500, 37)])
+def test_fp32_rows_get_all_of_the_sum(k, n, lengths, rank):
+    """Whole numbers: products up to 2^14, A x up to 2^23 (some 2^17), sums of B of them below 2^24 with entries of 0 and +-1 in B, eight of them
+    a column at most.  Nothing is rounded on the way in fp32, so out is exact: what is lost of A x shows."""
+    from ac4k_kernel_b200 import ops
+    y, x, a, b, offsets, adapters, _ = case(lengths, [i % 2 for i in range(len(lengths))], k, n, rank, 2, torch.float32)
+    g = torch.Generator().manual_seed(rank + k)
+    x = torch.randint(-128, 129, x.shape, generator=g).bfloat16().cuda()
+    a = torch.randint(-128, 129, a.shape, generator=g).bfloat16().cuda()
+    b = torch.randint(-1, 2, b.shape, generator=g).bfloat16().cuda()
+    b[:, :, 8:] = 0
+    y = torch.randint(-1000, 1000, y.shape, generator=g).float().cuda()
+    want, lo = y.double().clone(), offsets.tolist()
+    for i, j in enumerate(adapters.tolist()):
+        low = x[lo[i]:lo[i + 1]].double() @ a[j].double().t()
+        assert float(low.abs().max()) * 8 < 2 ** 24 - 1000
+        want[lo[i]:lo[i + 1]] += low @ b[j].double().t()
+    assert torch.equal(ops.lora(y, x, a, b, offsets, adapters).double(), want)
+
 
 @gpu
 @pytest.mark.parametrize("k,n", [(8, 8), (1, 1), (33, 65), (40, 200), (1000, 36), (4096, 1024), (5000, 1416), (130, 2050)])
@@ -154,6 +176,7 @@ def test_infinite_weights_give_infinities(exact, rank, dtype):
     assert torch.equal(out.isnan(), want.isnan())
     assert torch.equal(out == float("inf"), want == float("inf")) and torch.equal(out == -float("inf"), want == -float("inf"))
     assert bool(want.isinf().any()) and (not exact or bool(want.isnan().any()))
+
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
