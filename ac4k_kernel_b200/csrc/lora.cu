@@ -698,6 +698,7 @@ extern "C" int ac4k_lora(void *out, const void *y, int y_dtype, const void *x, c
   if (int e = lora::check_sizes(rows, requests, n_adapters, K, N, R)) return e;
   if (x_stride < 0 || y_stride < 0 || out_stride < 0) return fail(AC4K_ERR_SHAPE, "negative stride");
   if (rows == 0 || N == 0) return 0;
+  if (rows == 1) { x_stride = K; y_stride = out_stride = N; }         // (what one row's stride is means nothing)
   if (rows > 1 && out_stride < N) return fail(AC4K_ERR_SHAPE, "the rows of out overlap");
   if (!out || !y) return fail(AC4K_ERR_NULL, "a required pointer is NULL");
   const int size = y_dtype == AC4K_DT_FP32 ? 4 : 2;

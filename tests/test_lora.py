@@ -195,6 +195,28 @@ def test_strides(dtype, cut):
     wide = (y[:1, cut:cut + 240].expand(60, 240), *c[1:])           # one row of y for all
     check(ops.lora(*wide), *wide)
 
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n", [48, 45])
+def test_one_row_in_place_whatever_its_stride(n, dtype):
+    """A single row's stride means nothing: out at y's address is y"""
+    from ac4k_kernel_b200 import ops
+    y, x, a, b, offsets, adapters, s = case([1], [1], 64, n, 8, 2, dtype, seed=21)
+    want = ops.lora(y, x, a, b, offsets, adapters, s)
+    big = torch.full((3, 200), 7.0, dtype=dtype, device="cuda")
+    big[0, :n] = y[0]
+    out = big[0, :n].unsqueeze(0)
+    row = big[:1, :n].as_strided((1, n), (200, 1))
+    assert row.data_ptr() == out.data_ptr()
+    for given in (out.as_strided((1, n), (n, 1)), row, out.as_strided((1, n), (1, 1))):
+        big[0, :n] = y[0]
+        assert ops.lora(row, x, a, b, offsets, adapters, s, out=given) is given
+        assert torch.equal(given, want) and bool((big[0, n:] == 7).all())
+        assert torch.equal(ops.lora(row, x, a[:0], b[:0], offsets, adapters, out=given), want)
+    far = torch.zeros((1, 64), dtype=torch.bfloat16, device="cuda").as_strided((1, 64), (1, 1))      # one row of x, whatever its stride
+    far.copy_(x)
+    assert torch.equal(ops.lora(y, far, a, b, offsets, adapters, s), want)
+
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -387,3 +409,11 @@ def test_refusals_of_the_c_interface():
         assert last_error()
     assert call(t=0, out=None) == 0 and call(n=0) == 0
     assert call(out=P, y=P, l=0, x=None) == 0            # in place and nothing to add
+
+
+def test_one_row_in_place_is_not_refused():
+    from ac4k_kernel_b200._lib import LIB
+    P = 1 << 20
+    for strides in ((64, 64, 64), (64, 128, 64), (64, 64, 7), (1, 0, 0)):
+        assert LIB.ac4k_lora(P, P, 0, None, None, None, None, None, None, 1, 0, 0, 64, 64, 8, *strides, None) == 0, strides
+    assert LIB.ac4k_lora(P, P, 0, None, None, None, None, None, None, 2, 0, 0, 64, 64, 8, 64, 128, 64, None) == -2
