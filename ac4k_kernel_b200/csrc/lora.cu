@@ -707,16 +707,22 @@ extern "C" int ac4k_lora(void *out, const void *y, int y_dtype, const void *x, c
   if (out == y ? out_stride != y_stride : lora::rows_overlap(addr(out), out_stride * size, N * size, addr(y), y_stride * size, N * size, rows))
     return fail(AC4K_ERR_SHAPE, "out is y itself or does not overlap it");
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  if (n_adapters == 0 || requests == 0 || K == 0 || R == 0) {       // no adapter adds anything
-    if (rows > 1 && y_stride < N) return fail(AC4K_ERR_SHAPE, "the rows of y overlap");
-    auto pitch = [&](int64_t stride) { return (size_t)((stride < N ? N : stride) * size); };
-    if (out != y) AC4K_CUDA_TRY(cudaMemcpy2DAsync(out, pitch(out_stride), y, pitch(y_stride), (size_t)(N * size), (size_t)rows, cudaMemcpyDeviceToDevice, stream));
-    return 0;
+  const bool nothing = n_adapters == 0 || requests == 0 || K == 0 || R == 0;       // no adapter adds anything: y's rows as they are
+  if (nothing) {
+    if (rows > 1 && y_stride < N && y_stride != 0) return fail(AC4K_ERR_SHAPE, "the rows of y overlap");
+    if (out == y) return 0;
+    if (y_stride >= N && (y_stride > out_stride ? y_stride : out_stride) * size <= INT32_MAX) {       // (the longest pitch that there is)
+      AC4K_CUDA_TRY(cudaMemcpy2DAsync(out, (size_t)(out_stride * size), y, (size_t)(y_stride * size), (size_t)(N * size), (size_t)rows,
+                                      cudaMemcpyDeviceToDevice, stream));
+      return 0;
+    }
+    requests = K = R = 0;         // one row of y for all, or rows far apart: the kernel's copy of rows of no request
+  } else {
+    if (!x || !a || !b || !offsets || !adapters) return fail(AC4K_ERR_NULL, "a required pointer is NULL");
+    if (((addr(x) | addr(a) | addr(b)) & 1) || ((addr(offsets) | addr(adapters) | addr(scaling)) & 3)) return fail(AC4K_ERR_ALIGN, "a pointer is not aligned to its elements");
+    // (the columns of a row are written while other blocks still read their x)
+    if (lora::rows_overlap(addr(out), out_stride * size, N * size, addr(x), x_stride * 2, K * 2, rows)) return fail(AC4K_ERR_SHAPE, "out overlaps x");
   }
-  if (!x || !a || !b || !offsets || !adapters) return fail(AC4K_ERR_NULL, "a required pointer is NULL");
-  if (((addr(x) | addr(a) | addr(b)) & 1) || ((addr(offsets) | addr(adapters) | addr(scaling)) & 3)) return fail(AC4K_ERR_ALIGN, "a pointer is not aligned to its elements");
-  // (the columns of a row are written while other blocks still read their x)
-  if (lora::rows_overlap(addr(out), out_stride * size, N * size, addr(x), x_stride * 2, K * 2, rows)) return fail(AC4K_ERR_SHAPE, "out overlaps x");
   DeviceInfo di;
   if (int e = get_device_info(&di)) return e;
   lora::Args p = {};

@@ -30,6 +30,7 @@ __device__ __forceinline__ RaggedTile ragged_tile(const int32_t *__restrict__ of
   const int entries = groups + 2, per = (entries + THREADS - 1) / THREADS;
   auto bound = [&](int e) {        // where entry e begins; entry `entries` begins at the end
     if (e == 0) return 0;
+    if (groups == 0) return rows;  // (no offsets are read)
     return e == entries ? rows : min(max(__ldg(offsets + e - 1), 0), rows);
   };
   const int e0 = min((int)threadIdx.x * per, entries), e1 = min(e0 + per, entries);

@@ -274,8 +274,8 @@ int ac4k_rms_norm(void *out, void *sf, const float *global_scale, int precision,
  * reference).  The rows [offsets[i], offsets[i + 1]) are those of request i:
  *   out[t] = y[t] + scaling[j] * B_j (A_j x[t])  with j = adapters[i];  out[t] = y[t] where j is negative or no adapter (j >= n_adapters) and
  *   for rows in front of offsets[0] and behind offsets[requests].
- *   x: bf16 [rows, K], y and out: y_dtype [rows, N], all with contiguous rows that are *_stride elements apart; out is y itself (with its
- *   stride) or overlaps it nowhere.  a: bf16 [n_adapters, R, K], b: bf16 [n_adapters, N, R], dense; an adapter of a lower rank has zeros
+ *   x: bf16 [rows, K], y and out: y_dtype [rows, N], all with contiguous rows that are *_stride elements apart (one row of x or y for all: 0;
+ *   rows of y overlap in no other way); out is y itself (with its stride) or overlaps it nowhere.  a: bf16 [n_adapters, R, K], b: bf16 [n_adapters, N, R], dense; an adapter of a lower rank has zeros
  *   behind it.  offsets: int32 [requests + 1], ascending within [0, rows]; adapters: int32 [requests]; scaling: fp32 [n_adapters] or NULL
  *   (ones); all on the device.  R <= 128.
  * out does not overlap x either.  A x is held in fp32 and its product with B in fp32, with 16 bits of each value of A x for a bf16 or fp16 y and all of

@@ -294,6 +294,27 @@ def test_nothing_to_do():
     assert ops.lora(y[:0], x[:0], a, b, torch.zeros(3, dtype=torch.int32, device="cuda"), adapters).shape == (0, 48)
     assert ops.lora(y[:, :0].contiguous(), x, a, b[:, :0].contiguous(), offsets, adapters).shape == (8, 0)
 
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("t,n", [(8, 48), (8, 45), (1, 48), (200, 2056)])
+def test_one_row_of_y_for_all_without_an_adapter(t, n, dtype):
+    """Whether y may be one row for all does not hang on whether the batch has adapters, requests, features or a rank"""
+    from ac4k_kernel_b200 import ops
+    y, x, a, b, offsets, adapters, s = case([t // 2, t - t // 2], [0, 1], 64, n, 8, 2, dtype, seed=22)
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    for rows in (y[:1].expand(t, n), y, torch.cat([y, y], 1)[:, 3:3 + n]):
+        want = rows.contiguous()
+        big = torch.full((t + 2, n + 24), 7.0, dtype=dtype, device="cuda")
+        for out in (None, big[1:-1, 8:8 + n]):
+            for call in ((x, a, b, torch.zeros(1, dtype=torch.int32, device="cuda"), none), (x, a[:0], b[:0], offsets, adapters),
+                         (x, a[:, :0].contiguous(), b[:, :, :0].contiguous(), offsets, adapters, s),
+                         (x[:, :0].contiguous(), a[:, :, :0].contiguous(), b, offsets, adapters, s)):
+                got = ops.lora(rows, *call, out=out)
+                assert torch.equal(got, want)
+                got.fill_(3.0)
+        big[1:-1, 8:8 + n] = 7.0
+        assert bool((big == 7).all())
+
 
 @gpu
 def test_offsets_that_are_none():
