@@ -215,6 +215,26 @@ def test_rows_of_zeros_infinities_and_nan(k):
     q, sf = ops.rms_norm(x[:1], inf_w, precision="fp8e4m3")
     assert not sf[0].isfinite() and bool(q[0, 7].float().isnan())
 
+@gpu
+@pytest.mark.parametrize("k", [8, 24, 40, 72, 5128, 7, 61, 65, 1001, 5121])
+@pytest.mark.parametrize("rows", [6, 1030])
+def test_padding_is_zeros_beside_nan_and_infinities(k, rows):
+    """Rows whose scale is NaN or infinite: codes behind the last column are zeros all the same"""
+    from ac4k_kernel_b200 import ops
+    x, w, _ = inputs(rows, k, seed=k)
+    x[0, k - 1] = float("nan")
+    x[1, k // 2] = float("inf")
+    x[2, k - 1] = -float("inf")
+    x[3] = 0                           # with eps = 0 the formula's 0 / 0
+    for eps in (1e-6, 0.0):
+        q, sf = ops.rms_norm(x, w, eps, precision="fp8e4m3")
+        assert not q[:, k:].view(torch.uint8).any() and not sf[rows:].any()
+        assert bool(sf[:3].isnan().all()) and bool(sf[4:rows].isfinite().all()) and bool(sf[3] == 0 if eps else sf[3].isnan())
+        for layout in ("ac4k", "128x4"):
+            p, _, _ = ops.rms_norm(x, w, eps, precision="nvfp4", global_scale=torch.tensor(1.0 / 64, device="cuda"), sf_layout=layout)
+            codes = torch.stack((p & 15, p >> 4), -1).reshape(rows, -1)
+            assert not codes[:, k:].any()
+
 
 @gpu
 def test_no_rows():
