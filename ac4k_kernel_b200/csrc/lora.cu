@@ -472,8 +472,7 @@ lora_kernel(const lora::Args p) {
         const uint32_t at = p.slices > 1 ? ptx::map_to_cta(base + i * 4, q) : base + i * 4;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-          float4 d;
-          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(d.x), "=f"(d.y), "=f"(d.z), "=f"(d.w) : "r"(at + w * 16 * RP * 4) : "memory");
+          const float4 d = ptx::ld_shared_cluster_v4f(at + w * 16 * RP * 4);
           v.x += d.x; v.y += d.y; v.z += d.z; v.w += d.w;
         }
       }
@@ -487,7 +486,7 @@ lora_kernel(const lora::Args p) {
       }
       for (int q = 0; q < p.slices; ++q) {
         const uint32_t at = p.slices > 1 ? ptx::map_to_cta(total + i * 4, q) : total + i * 4;
-        asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
+        ptx::st_shared_cluster_v4u(at, u[0], u[1], u[2], u[3]);
       }
     }
     if (p.slices > 1) ptx::cluster_sync();              // behind this no block touches another's memory

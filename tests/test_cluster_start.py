@@ -32,3 +32,36 @@ def test_barrier_before_a_peers_shared_memory(file, name, body):
 def test_kernels_with_peers_are_found():
     assert {n for _, n, b in _kernels() if re.search(REMOTE, b)} >= {
         "nvfp4_quantize_flat_kernel", "linear_nvfp4_skinny_kernel", "linear_nvfp4_2cta_kernel"}
+
+
+# plain loads and stores, in either direction
+ACCESS = r"\b(st|ld)_shared_cluster_\w+\("
+
+
+def _stands_between(body):
+    """whether a cluster barrier stands in front of the first access to a peer's shared memory, and one behind the last"""
+    at = [m.start() for m in re.finditer(ACCESS, body)]
+    barriers = [m.start() for m in re.finditer(BARRIER, body)]
+    return bool(barriers) and barriers[0] < at[0] and barriers[-1] > at[-1]
+
+
+@pytest.mark.parametrize("file,name,body", [k for k in _kernels() if re.search(ACCESS, k[2])], ids=lambda v: v if len(v) < 60 else "")
+def test_barriers_around_loads_and_stores(file, name, body):
+    """A CTA that has left has no shared memory: the last access is behind a barrier that all pass as well"""
+    assert _stands_between(body), f"{file}: {name}"
+
+
+def test_no_access_goes_by_without_a_name():
+    """What these tests look for are the helpers' names, so no kernel writes the instructions out"""
+    for file, name, body in _kernels():
+        assert not re.search(r"\bshared::cluster\b|\bmapa\.", body), f"{file}: {name}"
+    assert {n for _, n, b in _kernels() if re.search(ACCESS, b)} >= {"lora_kernel", "nvfp4_quantize_flat_kernel"}
+
+
+def test_a_barrier_that_is_missing_is_seen():
+    body = {n: b for _, n, b in _kernels()}["lora_kernel"]
+    assert _stands_between(body)
+    calls = list(re.finditer(r"ptx::cluster_sync\(\)", body))
+    assert len(calls) == 2
+    for call in calls:
+        assert not _stands_between(body[:call.start()] + "__syncthreads()" + body[call.end():])
