@@ -310,7 +310,7 @@ linear_nvfp4_skinny_kernel(const __grid_constant__ CUtensorMap tma_x, const __gr
         if (m < p.M) st_shared_f32(scratch + m * 128 + lane * 4, __uint_as_float(r[m]));
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane < p.splits && lane != slice && rows_of(lane) > 0) {
+      if (tfull_ok && lane < p.splits && lane != slice && rows_of(lane) > 0) {      // (a slice that gave up sends nothing: nothing of it comes late)
         const int o = lane;
         const uint32_t unit = (uint32_t)(q * (p.splits - 1) + (slice < o ? slice : slice - 1)) * (uint32_t)rs * 128u;
         bulk_copy_to_cluster(map_to_cta(sPart + unit, o), scratch + (uint32_t)(o * rs) * 128u, (uint32_t)rows_of(o) * 128u,
@@ -320,8 +320,11 @@ linear_nvfp4_skinny_kernel(const __grid_constant__ CUtensorMap tma_x, const __gr
       const int rows = rows_of(slice);
       if (rows > 0) {
         const bool got = mbar_wait(part_bar + 8 * q, 0, p.wait_ns);
-        if (!got && lane == 0) atomicExch(p.status, kStatusTimeoutEpilogue);
-        if (n < p.N && tfull_ok) {
+        if (!got) {                 // a slice that is late may still send: one more limit for its copies to land before this memory is given up
+          if (lane == 0) atomicExch(p.status, kStatusTimeoutEpilogue);
+          mbar_wait(part_bar + 8 * q, 0, p.wait_ns);
+        }
+        if (n < p.N && tfull_ok && got) {
           const uint32_t own0 = scratch + (uint32_t)(slice * rs) * 128u + lane * 4;
           const uint32_t part0 = sPart + (uint32_t)(q * (p.splits - 1) * rs) * 128u + lane * 4;
           T *dst = static_cast<T *>(p.D) + (int64_t)(slice * rs) * p.N + n;

@@ -38,3 +38,18 @@ def test_waits_carry_the_limit_of_the_launch(path):
 @pytest.mark.parametrize("path", SOURCES, ids=os.path.basename)
 def test_no_grid_barrier_without_a_limit(path):
     assert not re.search(r"cooperative_groups|this_grid\(|grid_group", _code(path))
+
+
+@pytest.mark.parametrize("name", ["linear_nvfp4_skinny.cu", "linear_nvfp4_grouped.cu"])
+def test_no_copy_to_a_peer_outlives_an_expired_wait(name):
+    """The slices of a tile send one another their sums by bulk copies, which complete at the owner.  One that gave up on its own sum sends none, and an
+    owner whose wait ran out gives those of the others one more limit before it leaves: a copy never writes to, or reads from, the memory of a CTA
+    that has left.  What was not received is not stored."""
+    text = _code(os.path.join(CSRC, name))
+    sends = [m.start() for m in re.finditer(r"bulk_copy_to_cluster\(", text)]
+    assert len(sends) == 1
+    condition = text[text.rindex("if (", 0, sends[0]):sends[0]]
+    assert condition.startswith("if (tfull_ok && ")
+    behind = text[sends[0]:]
+    wait = re.search(r"const bool got = mbar_wait\((part_bar[^,]*), 0, p\.wait_ns\);\s*if \(!got\) \{[^}]*mbar_wait\(\1, 0, p\.wait_ns\);\s*\}\s*if \([^)]*&& got\)", behind)
+    assert wait and behind.index("cluster_sync_relaxed()") > wait.end()
