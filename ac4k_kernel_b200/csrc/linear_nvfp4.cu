@@ -654,8 +654,8 @@ using namespace ac4k;
 //   ac4k_debug_set_flags(bits)  8 skip the epilogue's stores; 64 launch without the
 //                               programmatic-stream-serialization attribute; 128 no L2 prefetch before the
 //                               dependency wait (pair kernel)
-//                               256 the pair kernel's producer leaves out the loads of its very first stage, so that
-//                               the waits for it expire (the wait-expiry test)
+//                               256 the producers of the pair kernels, and that of the first block of the grouped products', leave out the loads
+//                               of their very first stage, so that the waits for it expire (the wait-expiry test)
 //                               0x400 the last CTA of a tensor in the one-launch quantiser does not write its word, so that the
 //                               others' meeting expires
 //                               0x800 the last CTA of a tensor there begins to load one and a half limits late, when the waits for

@@ -58,6 +58,7 @@ struct Args {
   int tiles_n, splits, kt_per_split;
   bool fill;                     // write zeros to the rows of no group
   unsigned long long wait_ns;
+  int dbg;                       // experiment switches (builds with -DAC4K_DEBUG_HOOKS), else 0
 };
 
 // alpha and bias of a weight row (output column) of group e
@@ -181,6 +182,10 @@ linear_nvfp4_grouped_kernel(const __grid_constant__ CUtensorMap tma_x, const __g
     for (int kt = kt0; kt < kt1; ++kt) {
       ok = warp_all(mbar_wait(empty_bar + 8 * s, ph ^ 1, p.wait_ns));
       if (!ok) break;
+      if (AC4K_DBG(p, 256) && kt == kt0 && blockIdx.x == 0) {        // wait-expiry test: this stage's operands never come
+        if (++s == STAGES) { s = 0; ph ^= 1; }
+        continue;
+      }
       const uint32_t fb = full_bar + 8 * s;
       mbar_arrive_expect_tx_if(el, fb, W_BYTES + C::X_BYTES);
       tma_load_2d_if(el, sW + s * W_BYTES, &tma_w, kt * BKB, w_row, fb);
@@ -461,6 +466,7 @@ extern "C" int ac4k_linear_nvfp4_grouped(void *D, int d_dtype, const void *A, co
   a.kt_per_split = (int)ceil_div(k_tiles, splits);
   a.fill = fill != 0;
   a.wait_ns = debug_wait_ns() ? debug_wait_ns() : kWaitTimeoutNs;
+  a.dbg = debug_flags();
   const int64_t blocks = tiles * tiles_n * splits;
   switch (nt) {
     case 16: return launch_grouped_dt<16>(d_dtype, tx, tw, a, blocks, stream);

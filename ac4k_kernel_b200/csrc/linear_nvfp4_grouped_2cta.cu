@@ -41,6 +41,7 @@ struct Args {
   bool fill;
   bool wide;                     // rows of D begin on 32 bytes
   unsigned long long wait_ns;
+  int dbg;                       // experiment switches (builds with -DAC4K_DEBUG_HOOKS), else 0
 };
 
 struct TileOf {
@@ -195,6 +196,10 @@ linear_nvfp4_grouped_2cta_kernel(const __grid_constant__ CUtensorMap tma_a, cons
         ok = warp_all(mbar_wait(empty_bar + 8 * s, ph ^ 1, p.wait_ns));
         if (!ok) break;
         const uint32_t lf = leader_full0 + 8 * s;
+        if (AC4K_DBG(p, 256) && kt == 0 && t == cluster_id) {       // wait-expiry test: the first stage of each pair never comes
+          if (++s == STAGES) { s = 0; ph ^= 1; }
+          continue;
+        }
         // the leader announces the bytes of both CTAs; rows and K steps past the end of a tensor arrive as zeros (K steps past the end of
         // this group's as the next one's scales, unused) and count all the same
         if (rank == 0) mbar_arrive_expect_tx_if(el, full_bar + 8 * s, tx);
@@ -419,6 +424,7 @@ int launch_linear_grouped_pair(void *D, int d_dtype, const void *A, const void *
   a.fill = fill;
   a.wide = N % 16 == 0 && (reinterpret_cast<uintptr_t>(D) & 31) == 0;
   a.wait_ns = wait_ns;
+  a.dbg = debug_flags();
   if (a.row_classes == 4) ta_hi = ta;
   // row tiles of a group of n rows that begins up to three rows early: at most (n + 3) / 256 + 1
   const int64_t used = groups < M ? groups : M, most = (ceil_div(M + 3 * used, pair::BMP) + used) * a.tiles_n;

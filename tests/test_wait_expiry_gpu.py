@@ -106,3 +106,47 @@ def test_expired_waits_of_the_one_launch_quantiser(shape, cross, reduce, swizzle
     for a, b in zip(got, want):
         assert torch.equal(a.reshape(-1).view(torch.uint8), b.reshape(-1).view(torch.uint8))
     assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("lengths,n,k,dtype", [([5, 3], 256, 4096, torch.bfloat16),         # four slices of K, whose sums meet
+                                               ([5, 3], 256, 2048, torch.bfloat16),         # two
+                                               ([9, 0, 12], 200, 512, torch.float16),       # one
+                                               ([50, 40], 136, 320, torch.float32),         # tiles of 64 rows
+                                               ([100, 150], 136, 512, torch.float32),       # of 128
+                                               ([300, 200], 520, 512, torch.bfloat16),      # CTA pairs
+                                               ([301, 0, 1200], 520, 2048, torch.float16)], ids=str)
+def test_expired_waits_of_the_grouped_products(lengths, n, k, dtype):
+    """The first stage of a block, or of every pair, is never loaded: its MMA issuer gives up, then the roles behind it and the slices that wait for its sum.  The
+    status says so, every block leaves, and the next call is right.  What was not computed is not stored."""
+    from ac4k_kernel_b200 import _lib, ops
+    hooks = hooks_library()
+    m, e = sum(lengths), len(lengths)
+    x, x_sf, x_g = ops.quantize(gaussian((m, k), seed=7).cuda(), 0, 1)
+    w, w_sf, w_g = ops.quantize(gaussian((e, n, k), seed=8, std=0.05).cuda(), 1, 2)
+    offsets = torch.tensor([sum(lengths[:i]) for i in range(e + 1)], dtype=torch.int32, device="cuda")
+    want = ops.linear_grouped(x, x_sf, x_g, w, w_sf, w_g, offsets, out=torch.empty((m, n), dtype=dtype, device="cuda"))
+    code = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}[dtype]
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def grouped(out):
+        return hooks.ac4k_linear_nvfp4_grouped(out.data_ptr(), code, x.data_ptr(), x_sf.data_ptr(), x_g.data_ptr(), w.data_ptr(), w_sf.data_ptr(), w_g.data_ptr(), 0,
+                                               None, 0, offsets.data_ptr(), 0, m, e, n, k, stream)
+
+    status = ctypes.c_uint32(0)
+    assert hooks.ac4k_device_status(ctypes.byref(status), 1) == 0 and status.value == 0
+    out = torch.full((m, n), 7.0, dtype=dtype, device="cuda")
+    try:
+        hooks.ac4k_debug_set_wait_ns(3_000_000)
+        hooks.ac4k_debug_set_flags(256)
+        assert grouped(out) == 0
+        rc = hooks.ac4k_device_status(ctypes.byref(status), 1)
+    finally:
+        hooks.ac4k_debug_set_flags(0)
+        hooks.ac4k_debug_set_wait_ns(0)
+    assert rc == -7 and status.value in (0xA1, 0xA2, 0xA3, 0xA4), (rc, hex(status.value))
+    assert b"bounded device-side wait expired" in hooks.ac4k_last_error()
+    assert bool(((out == want) | (out == 7)).all()) and bool((out == 7).any())
+    assert grouped(out) == 0
+    assert hooks.ac4k_device_status(ctypes.byref(status), 1) == 0 and status.value == 0
+    assert torch.equal(out, want)
+    assert torch.equal(ops.linear_grouped(x, x_sf, x_g, w, w_sf, w_g, offsets, out=torch.empty_like(out)), want) and _lib.device_status() == 0
