@@ -193,6 +193,31 @@ def test_offsets_that_are_none(t, behind):
         torch.cuda.synchronize()
         assert bool((big[:behind] == 7).all()) and bool((big[behind + rows:] == 7).all())
 
+@gpu
+@pytest.mark.parametrize("n", [136, 520])
+@pytest.mark.parametrize("fill", [False, True])
+def test_offsets_that_are_none_in_pairs(n, fill):
+    """As above, at widths and lengths of the CTA-pair kernel, which has its own lookup; lists without any row among them"""
+    from ac4k_kernel_b200 import _cuda_ops, _lib, ops
+    x, x_sf, x_g, w, w_sf, w_g, right = case([250, 0, 200, 250], n, 256, seed=23)
+    rows, behind = x.shape[0], 60
+    big = torch.full((rows + 2 * behind, n), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = big[behind:behind + rows]
+    if out.data_ptr() % 16:
+        pytest.fail("the rows begin on 16 bytes")
+    want = ops.linear_grouped(x, x_sf, x_g, w, w_sf, w_g, right)
+    for bad in ([-5, 10, 20, 30, rows], [0, 10, 20, 10 ** 6, 10 ** 6], [0, 20, 10, 30, 30], [30, 20, 10, 0, 5], [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, 5, 9],
+                [0, rows, 0, rows, 0], [rows] * 5, [0] * 5, [300] * 5, [-7] * 5):
+        out.fill_(5.0)
+        offsets = torch.tensor(bad, dtype=torch.int32, device="cuda")
+        _cuda_ops.linear_nvfp4_grouped(out, x, x_sf, x_g, w, w_sf, w_g, offsets, None, fill)
+        assert _lib.device_status() == 0
+        assert bool((big[:behind] == 7).all()) and bool((big[behind + rows:] == 7).all())
+        if len(set(bad)) == 1:                          # no group has a row
+            assert bool((out == (0.0 if fill else 5.0)).all())
+    _cuda_ops.linear_nvfp4_grouped(out, x, x_sf, x_g, w, w_sf, w_g, right, None, fill)
+    assert torch.equal(out, want)
+
 
 @gpu
 def test_same_result_each_time_streams_and_graphs():
