@@ -166,6 +166,33 @@ def test_many_groups():
     c = case(lengths, 64, 64, lead=2, behind=1, seed=17)
     check(ops.linear_grouped(*c), *c)
 
+@gpu
+@pytest.mark.parametrize("lead,behind", [(0, 0), (3, 5)])
+@pytest.mark.parametrize("groups,longest", [(129, 60), (300, 40), (700, 30)])
+def test_more_groups_than_ranges_of_the_table(groups, longest, lead, behind):
+    """The CTA-pair kernel's table has 128 entries: several groups an entry, empty ones among them"""
+    from ac4k_kernel_b200 import ops
+    g = torch.Generator().manual_seed(groups)
+    lengths = torch.randint(-longest // 8, longest + 1, (groups,), generator=g).clamp(min=0).tolist()
+    assert sum(lengths) > 9 * groups             # (what sends them to the pairs at this K)
+    c = case(lengths, 264, 256, lead, behind, seed=groups)
+    out = torch.full((c[0].shape[0], 264), 7.0, dtype=torch.bfloat16, device="cuda")
+    check(ops.linear_grouped(*c, out=out), *c)
+    rest = torch.ones(out.shape[0], dtype=torch.bool, device="cuda")
+    rest[lead:lead + sum(lengths)] = False
+    assert bool((out[rest] == 7).all())
+    assert not ops.linear_grouped(*c)[rest].any()
+
+@gpu
+@pytest.mark.parametrize("groups,each", [(200, 30), (3, 20000)])
+def test_more_tiles_than_are_listed(groups, each):
+    """More than 48 tiles of 256 x 256 for each of 74 pairs (3552): the rest are looked up as they come"""
+    from ac4k_kernel_b200 import ops
+    lengths = [each + i % 3 for i in range(groups)]
+    c = case(lengths, 8192, 64, seed=each)
+    assert groups * -(-each // 256) * 32 > 3552
+    check(ops.linear_grouped(*c), *c)
+
 
 @gpu
 def test_nothing_to_do():
