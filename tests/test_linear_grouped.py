@@ -122,6 +122,18 @@ def test_groups_that_fill_half_a_tile(lengths, n, k, dtype):
     check(ops.linear_grouped(*c, out=out), *c)
     assert bool((out[:1] == 7).all()) and bool((out[-2:] == 7).all())
 
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lengths", [[100, 100, 0, 100], [129, 201, 63, 127], [125, 3, 128, 259], [385, 380, 1, 0], [53] * 40, [256, 256, 257, 511]], ids=str)
+@pytest.mark.parametrize("n,k", [(136, 576), (264, 960)])
+def test_groups_that_fill_half_a_tile_uncut(lengths, n, k, dtype):
+    """As above with a K that is not cut into slices (fewer than eight stages of 256), so that all of them are tiles of CTA pairs"""
+    from ac4k_kernel_b200 import ops
+    c = case(lengths, n, k, lead=1, behind=2, seed=n + len(lengths))
+    out = torch.full((c[0].shape[0], n), 7.0, dtype=dtype, device="cuda")
+    check(ops.linear_grouped(*c, out=out), *c)
+    assert bool((out[:1] == 7).all()) and bool((out[-2:] == 7).all())
+
 
 @gpu
 def test_a_group_is_the_same_alone_and_among_others():

@@ -92,6 +92,17 @@ def test_clusters_of_every_size(lengths, rank):
     c = case(lengths, [i % 3 for i in range(len(lengths))], 4872, 4424, rank, 3, seed=rank + len(lengths))
     check(ops.lora(*c), *c)
 
+@gpu
+@pytest.mark.parametrize("rank", [16, 32, 64, 128])
+@pytest.mark.parametrize("tiles", [56, 72, 95, 108, 140, 190, 220, 290, 400])
+def test_clusters_of_few_blocks(tiles, rank):
+    """A prompt of so many tiles of 64 rows that a cluster has 1 to 5 blocks, or more of them where four fit on an SM: 148 SMs hold 592 blocks of ranks 16 and
+    32, 444 of rank 64 and 296 of rank 128"""
+    from ac4k_kernel_b200 import ops
+    lengths = [64 * tiles - 70, 0, 33]
+    c = case(lengths, [0, 1, 1], 1304, 1288, rank, 2, lead=2, seed=tiles)
+    check(ops.lora(*c), *c)
+
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
