@@ -240,4 +240,12 @@ __device__ __forceinline__ float amax16_bf16(const uint32_t *w) {
   return hmax_bf16x2_to_f32(m);
 }
 
+// Whether two sets of rows share a byte (strides and lengths in bytes).  Rows of one stride may lie between each other.
+inline bool rows_overlap(uintptr_t a, int64_t a_stride, int64_t a_len, uintptr_t b, int64_t b_stride, int64_t b_len, int64_t rows) {
+  if (a >= b + (rows - 1) * b_stride + b_len || b >= a + (rows - 1) * a_stride + a_len) return false;
+  if (rows == 1 || a_stride != b_stride || a_stride == 0) return true;
+  const int64_t d = (int64_t)(b - a) % a_stride, behind = d < 0 ? d + a_stride : d;       // where b's rows begin behind a's
+  return behind < a_len || behind + b_len > a_stride;
+}
+
 }  // namespace ac4k

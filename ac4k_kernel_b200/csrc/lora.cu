@@ -669,14 +669,6 @@ static int launch_tm(const Args &p, int dt, int sms, cudaStream_t stream) {
   return launch_dtype<TM, 128>(p, dt, sms, stream);
 }
 
-// Whether two sets of rows share a byte (strides and lengths in bytes).  Rows of one stride may lie between each other.
-static bool rows_overlap(uintptr_t a, int64_t a_stride, int64_t a_len, uintptr_t b, int64_t b_stride, int64_t b_len, int64_t rows) {
-  if (a >= b + (rows - 1) * b_stride + b_len || b >= a + (rows - 1) * a_stride + a_len) return false;
-  if (rows == 1 || a_stride != b_stride || a_stride == 0) return true;
-  const int64_t d = (int64_t)(b - a) % a_stride, behind = d < 0 ? d + a_stride : d;       // where b's rows begin behind a's
-  return behind < a_len || behind + b_len > a_stride;
-}
-
 static int check_sizes(int64_t rows, int64_t requests, int64_t adapters, int64_t K, int64_t N, int64_t R) {
   if (rows < 0 || requests < 0 || adapters < 0 || K < 0 || N < 0 || R < 0) return fail(AC4K_ERR_SHAPE, "negative size");
   if (rows > (1 << 30) || requests > (1 << 24) || adapters > (1 << 24) || K > (1 << 24) || N > (1 << 22))
@@ -703,7 +695,7 @@ extern "C" int ac4k_lora(void *out, const void *y, int y_dtype, const void *x, c
   const int size = y_dtype == AC4K_DT_FP32 ? 4 : 2;
   auto addr = [](const void *q) { return reinterpret_cast<uintptr_t>(q); };
   if ((addr(y) | addr(out)) & (size - 1)) return fail(AC4K_ERR_ALIGN, "y or out is not aligned to its elements");
-  if (out == y ? out_stride != y_stride : lora::rows_overlap(addr(out), out_stride * size, N * size, addr(y), y_stride * size, N * size, rows))
+  if (out == y ? out_stride != y_stride : rows_overlap(addr(out), out_stride * size, N * size, addr(y), y_stride * size, N * size, rows))
     return fail(AC4K_ERR_SHAPE, "out is y itself or does not overlap it");
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   const bool nothing = n_adapters == 0 || requests == 0 || K == 0 || R == 0;       // no adapter adds anything: y's rows as they are
@@ -720,7 +712,7 @@ extern "C" int ac4k_lora(void *out, const void *y, int y_dtype, const void *x, c
     if (!x || !a || !b || !offsets || !adapters) return fail(AC4K_ERR_NULL, "a required pointer is NULL");
     if (((addr(x) | addr(a) | addr(b)) & 1) || ((addr(offsets) | addr(adapters) | addr(scaling)) & 3)) return fail(AC4K_ERR_ALIGN, "a pointer is not aligned to its elements");
     // (the columns of a row are written while other blocks still read their x)
-    if (lora::rows_overlap(addr(out), out_stride * size, N * size, addr(x), x_stride * 2, K * 2, rows)) return fail(AC4K_ERR_SHAPE, "out overlaps x");
+    if (rows_overlap(addr(out), out_stride * size, N * size, addr(x), x_stride * 2, K * 2, rows)) return fail(AC4K_ERR_SHAPE, "out overlaps x");
   }
   DeviceInfo di;
   if (int e = get_device_info(&di)) return e;

@@ -485,6 +485,16 @@ extern "C" int ac4k_rms_norm(void *out, void *sf, const float *global_scale, int
   if ((addr(x) & 1) || (addr(residual) & (rsize - 1)) || (addr(residual_out) & (rsize - 1)) || (addr(weight) & (wsize - 1)) || (addr(normed) & 1) ||
       (addr(out) & (precision == AC4K_NORM_BF16 ? 1 : 3)) || (addr(sf) & 3) || (addr(global_scale) & 3))
     return fail(AC4K_ERR_ALIGN, "a pointer is not aligned to its elements");
+  if (M == 1) x_stride = residual_stride = K;            // (what one row's stride is means nothing)
+  if (residual_out) {
+    // each element is read and written by one thread where the rows coincide; any other overlap has rows read after they were written
+    auto meets = [&](const void *q, int64_t stride, int size) {
+      return q && rows_overlap(addr(residual_out), K * rsize, K * rsize, addr(q), stride * size, K * size, M);
+    };
+    if ((meets(x, x_stride, 2) && !(residual_out == x && x_stride == K && rsize == 2)) ||
+        (meets(residual, residual_stride, rsize) && !(residual_out == residual && residual_stride == K)))
+      return fail(AC4K_ERR_SHAPE, "residual_out is the residual or x itself, element by element, or overlaps neither");
+  }
   norm::Args p = {};
   p.x = static_cast<const uint16_t *>(x);
   p.residual = residual;

@@ -344,3 +344,20 @@ def test_refusals_of_the_c_interface():
         assert last_error()
     assert call(m=0, out=None) == 0
     assert isinstance(LIB.ac4k_rms_norm, ctypes._CFuncPtr)
+
+
+def test_residual_out_that_overlaps_is_refused():
+    """residual_out is the residual or x itself, in the same places and of the same type, or overlaps neither (no GPU: the refusal comes first)"""
+    from ac4k_kernel_b200._lib import LIB, last_error
+    Q = 1 << 20
+
+    def call(residual_out, x=Q, residual=4 * Q, rdt=0, m=4, k=64, xs=64, rs=64):
+        return LIB.ac4k_rms_norm(8 * Q, 9 * Q, 10 * Q, 2, 0, None, residual_out, x, residual, rdt, None, 0, 1e-6, m, k, xs, rs, None)
+
+    for kw in (dict(residual_out=Q, xs=128), dict(residual_out=Q, rdt=2), dict(residual_out=Q + 128), dict(residual_out=Q - 128), dict(residual_out=4 * Q, rs=65),
+               dict(residual_out=4 * Q, rs=0), dict(residual_out=4 * Q + 16), dict(residual_out=4 * Q + 256, rdt=2), dict(residual_out=Q, rdt=2, m=1)):
+        assert call(**kw) == -2 and "residual_out" in last_error(), kw
+    if not torch.cuda.is_available():          # past the checks: there is no device to launch on
+        for kw in (dict(residual_out=Q), dict(residual_out=4 * Q), dict(residual_out=4 * Q, rdt=2), dict(residual_out=Q, xs=999, m=1), dict(residual_out=4 * Q, rs=7, m=1),
+                   dict(residual_out=Q + 512, xs=64), dict(residual_out=2 * Q)):
+            assert call(**kw) > 0, kw
