@@ -10,8 +10,11 @@
 // multiplied with this group's weight there and not stored.  (Narrower or shifted tiles would need the scales re-ordered by threads, which
 // costs the tensor pipe 12 - 30 % of every stage.)
 //
-// Bound by what L2 hands to the SMs: a stage of a pair is 58 to 76 KB for 520 cycles of MMAs.  16384 rows of 8 groups, 8192 x 4096: 250 us (4.4 PFLOP/s,
-// 10.3 TB/s from L2); 4099 rows of 48 groups, 2048 x 2048: 34.5 us (117 MB, 3.4 TB/s; 5.2 rounds of tiles run as 6).
+// Large groups are bound as the plain kernel is, by the tensor pipe and by power.  16384 rows, 8192 x 4096, calls one after another (1000 W, SM clock 1390
+// to 1510 MHz): 274 us for 8 even groups, 285 for uneven ones, 262 for `linear` with one weight; a call by itself at 1965 MHz 235, 244 and 242.  The tensor
+// pipe is busy 67 % of the cycles (64 % in `linear`), L2 44 %.  Uneven groups end in row tiles that other groups' rows fill up: 4 %.
+// Short groups are bound by such tiles: 4099 rows of 48 groups, 2048 x 2048, 39.5 us, are 385 tiles for rows that fill 129, 5.2 rounds run as 6; a stage
+// (58 KB to a pair) takes 700 to 1000 cycles where its MMAs take 520.
 #include "linear_nvfp4_pair.cuh"
 
 namespace ac4k {

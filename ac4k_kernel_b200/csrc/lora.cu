@@ -2,8 +2,9 @@
 //
 //   out[t] = y[t] + scaling[a] * B_a (A_a x[t]),   a = adapters[request of row t], or none: out[t] = y[t]
 //
-// A rank of 8 to 128 makes 2 R operations per byte of x and of y, below what the memory allows for up to R = 64: the work is to read x, y and the
-// adapters once and to write out once.  One launch: a cluster of up to 16 blocks takes a tile of rows of one request.  Each block sums A x over its
+// A row takes 2 R (K + N) operations and, in bf16, 2 K + 4 N bytes: with K = N 2 R / 3 operations a byte, 85 for R = 128 (128 with the second half's two
+// MMAs each), where the tensor pipe and the memory meet at 253 (tcgen05; 1.66 PFLOP/s, 6.55 TB/s).  So the work is to read x, y and the adapters once and
+// to write out once; what these kernels reach of that is a matter of latency (29 % of the issue slots, tensor pipe 35 % at rank 64).  One launch: a cluster of up to 16 blocks takes a tile of rows of one request.  Each block sums A x over its
 // slice of K ("shrink"), the blocks add their sums in order through distributed shared memory (no atomics, the same result each time), and each
 // adds B of that to its slice of y's columns ("expand").  Nothing goes through global memory in between, and the second half's first operands
 // are on their way while the sums are exchanged.  (As two launches with A x in a workspace: 15.7 us for 64 requests of one token, rank 16,
@@ -729,7 +730,9 @@ extern "C" int ac4k_lora(void *out, const void *y, int y_dtype, const void *x, c
   p.b_vec = R % 8 == 0 && (addr(b) & 15) == 0;
   const int lanes = 16 / size;
   p.y_vec = N % 8 == 0 && y_stride % lanes == 0 && out_stride % lanes == 0 && ((addr(y) | addr(out)) & 15) == 0;
-  // tiles of 64 rows where a request has 32 or more on average, else of 16
+  // Tiles of 64 rows where a request has 32 or more on average, else of 16.  (The lengths are on the device.  A long request among short ones goes
+  // in tiles of 16, which read its adapter anew each: 2000 rows and 127 of one, 4096 x 4096, 20.8 us at rank 16 and 50.7 at rank 64; in two calls, 11.0 + 15.8
+  // and 20.8 + 24.3, so at rank 64 two are faster.)
   if (rows >= 32 * requests) return lora::launch_tm<64>(p, y_dtype, di.sms, stream);
   return lora::launch_tm<16>(p, y_dtype, di.sms, stream);
 }

@@ -144,7 +144,9 @@ __device__ __forceinline__ void reduce_row(float &sum, float &amax, float *part)
 namespace norm {
 // Blocks on an SM that the compiler is to leave registers for: as many rows in flight as a row's 8 C values and its two loads of 4 C words allow.
 // Left to itself it took 86 registers for C = 5, and 4099 rows of 5120 (bf16 residual, e4m3 out) 28.3 us, now 27.4; without a residual 20.9 and 19.0; 6144
-// 37.0 and 35.2; 12288 69.1 and 62.8.  (8 blocks for C = 5 spill: 29.2.)
+// 37.0 and 35.2; 12288 69.1 and 62.8.  (8 blocks for C = 5 spill: 29.2.  All back to back, over four inputs in turn; a call among calls on new inputs each
+// takes 29.7.)  Bytes and time of the other forms of 4099 x 5120: bf16 out 168 MB 27.6 us, NVFP4 138 MB 26.6; with an fp32 residual e4m3 231 MB 43.6, NVFP4
+// 222 MB 47.8.
 constexpr int blocks_for(int c, int threads) {
   return c == 8 ? 512 / threads : (c == 6 ? 768 / threads : (c == 5 ? 896 / threads : (c == 4 ? 1024 / threads : 1)));
 }
@@ -305,8 +307,8 @@ rms_norm_kernel(const norm::Args p) {
 
 // Any K, stride and alignment: a block of T threads per row, the row as fp32 in shared memory.  x, the residual and outputs of the same width go by single
 // elements, neighbours by neighbouring threads, a batch of loads in front of its first use; the quantised row begins on 16 bytes
-// and goes by four elements a thread.  Threads by K: 30000 rows of 1001 (bf16 residual, e4m3 out) take 106 us, 299 with 512 threads a row; 9999 rows of
-// 11003 take 430 us (1.8 TB/s: seven loads and stores of a warp for every 32 elements), 461 with an element and a code at a time.
+// and goes by four elements a thread.  Threads by K: 30000 rows of 1001 (bf16 residual, e4m3 out) take 107 us, 299 with 512 threads a row; 9999 rows of
+// 11003 take 427 us (1.8 TB/s: seven loads and stores of a warp for every 32 elements), 461 with an element and a code at a time.
 template <int FMT, int T>
 __global__ void __launch_bounds__(T)
 rms_norm_any_kernel(const norm::Args p) {

@@ -76,7 +76,8 @@ def linear_grouped(x, x_scale, x_global_scale, weight, weight_scale, weight_glob
     counterpart): out[t] = x[t] @ weight[e].T + bias[e] for the rows offsets[e] to offsets[e + 1].
 
     x, x_scale, x_global_scale: what `quantize(rows, 0, 1)` returns for all rows together, packed [M, K/2] u8, [K/64, align_up(M, 16), 4] e4m3,
-    0-dim; weight, weight_scale: `quantize(weights, 1, 2)` of the [E, N, K] weights, [E, N, K/2] u8, [E, K/64, align_up(N, 16), 4] e4m3;
+    0-dim; weight, weight_scale: `quantize(weights, 1, 2)` of the [E, N, K] weights, [E, N, K/2] u8, [E, K/64, align_up(N, 16), 4] e4m3
+    (scales in the row layout, `quantize()`'s and `rms_norm()`'s default; 128x4 tiles are refused);
     weight_global_scale: 0-dim, or [E] where each weight was quantised by itself; offsets: int32 [E + 1], ascending; bias: [E, N]
     bf16/fp16/fp32; out: optional [M, N] bf16/fp16/fp32.  A group may be empty.  Rows of no group (in front of offsets[0] or behind
     offsets[E]) are zeros in an output that is allocated here and left as they are in one that is given.  Returns out."""

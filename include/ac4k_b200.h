@@ -264,7 +264,8 @@ int ac4k_rope3d(void *out, const void *x, const int32_t *grid_sizes, const void 
  *   with block scales sf in `sf_layout` for the given global scale (what ac4k_linear_nvfp4 takes).  Padding is written as zeros.
  *   normed: NULL, or v in bf16 [M, K] beside a quantised out.  residual_out: NULL or [M, K] of residual_dtype; it may be the residual
  *   itself (residual_stride = K) or x (x_stride = K, bf16), and overlaps no tensor of the call otherwise.
- * A quantised out begins on 4 bytes.  K <= 32768.  Sums of squares past fp32's range (elements of 1e17 and more) give zeros, as infinity under the root does. */
+ * A quantised out begins on 4 bytes.  K <= 32768.  Sums of squares past fp32's range (elements of 1e17 and more) give zeros, as infinity under the root does;
+ * with eps = 0 a row whose squares vanish in fp32 (no element of 2^-75 and more) gives infinities or NaN, as the root of 0 does. */
 enum { AC4K_NORM_BF16 = 0, AC4K_NORM_E4M3 = 1, AC4K_NORM_NVFP4 = 2 };
 int ac4k_rms_norm(void *out, void *sf, const float *global_scale, int precision, int sf_layout, void *normed, void *residual_out,
                   const void *x, const void *residual, int residual_dtype, const void *weight, int weight_dtype, float eps,
